@@ -104,6 +104,7 @@ struct Model {
   std::vector<float*> acts;  // inputs of each layer (acts[l]) and the final output
   int64_t part_cap = 0;
   int64_t launches = 0;
+  bool have_tape = false;  // a forward's residual is in the handle
   std::vector<void*> owned;
 
   void* alloc(size_t bytes) {
@@ -143,12 +144,10 @@ struct Model {
     for (void* p : owned) cudaFree(p);
   }
 
+  // get: tokens -> logits, the residual kept in the blocks, acts and h_act
   template <typename Act>
-  void run(const Act* P, const int64_t* tokens, const int64_t* targets, float* loss, float* dP,
-           float* logits_out, cudaStream_t s) {
+  void forward(const Act* P, const int64_t* tokens, float* logits_to, cudaStream_t s) {
     const int64_t D = cfg.dim, V = cfg.vocab, L = cfg.layers;
-    const bool f32 = std::is_same<Act, float>::value;
-    DOP_CHECK_CUDA(cudaMemsetAsync(dP, 0, sizeof(float) * total, s));  // a fresh adjoint
     k_embed<Act><<<(unsigned)T, 256, 0, s>>>(P + embed, tokens, (int)D, acts[0]);
     DOP_LAUNCHED(launches);
     for (int64_t l = 0; l < L; ++l)
@@ -157,8 +156,16 @@ struct Model {
     rmsnorm_fwd<Act>(acts[L], P + final_norm, T, (int)D, cfg.rms_eps, (Act*)h_act, h_inv, nullptr,
                      s, launches);
     Gemm gh; gh.M = T; gh.N = V; gh.K = D; gh.A = h_act; gh.lda = D; gh.B = P + lm_head;
-    gh.ldb = V; gh.C = logits; gh.ldc = V;
+    gh.ldb = V; gh.C = logits_to; gh.ldc = V;
     gemm(gh, s);
+    have_tape = true;
+  }
+
+  template <typename Act>
+  void run(const Act* P, const int64_t* tokens, const int64_t* targets, float* loss, float* dP,
+           float* logits_out, cudaStream_t s) {
+    const int64_t V = cfg.vocab;
+    forward<Act>(P, tokens, logits, s);
     k_cross_entropy<<<(unsigned)T, 256, 0, s>>>(logits, targets, T, (int)V, row_loss, dlogits);
     DOP_LAUNCHED(launches);
     k_mean_loss<<<1, 32, 0, s>>>(row_loss, T, loss);
@@ -166,10 +173,19 @@ struct Model {
     if (logits_out)
       DOP_CHECK_CUDA(cudaMemcpyAsync(logits_out, logits, sizeof(float) * T * V,
                                      cudaMemcpyDeviceToDevice, s));
-    // backward (src/mixtral.rs:382-432)
-    const void* dl_op = dlogits;
-    if (!f32) {
-      convert<Act>(dlogits, (Act*)dlogits_act, T * V, s, launches);
+    backward<Act>(P, tokens, dlogits, DOP_F32, dP, s);
+  }
+
+  // put (src/mixtral.rs:382-432): dlogits in grad_prec -> a fresh adjoint dP
+  template <typename Act>
+  void backward(const Act* P, const int64_t* tokens, const void* dlogits_in, int grad_prec,
+                float* dP, cudaStream_t s) {
+    const int64_t D = cfg.dim, V = cfg.vocab, L = cfg.layers;
+    const bool f32 = std::is_same<Act, float>::value;
+    DOP_CHECK_CUDA(cudaMemsetAsync(dP, 0, sizeof(float) * total, s));  // a fresh adjoint
+    const void* dl_op = dlogits_in;
+    if (!f32 && grad_prec == DOP_F32) {
+      convert<Act>((const float*)dlogits_in, (Act*)dlogits_act, T * V, s, launches);
       dl_op = dlogits_act;
     }
     Gemm gd; gd.M = T; gd.N = D; gd.K = V; gd.A = dl_op; gd.lda = V; gd.B = P + lm_head;
@@ -239,6 +255,35 @@ int dop_model_forward_backward(dop_model* m_, const void* params, const int64_t*
       m->run<float>((const float*)params, tokens, targets, loss, dparams, logits, s);
     else
       m->run<dop::bf16>((const dop::bf16*)params, tokens, targets, loss, dparams, logits, s);
+  })
+}
+
+int dop_model_forward(dop_model* m_, const void* params, const int64_t* tokens, float* logits,
+                      void* stream) {
+  DOP_MODEL_GUARD({
+    DOP_REQUIRE(m_ && params && tokens && logits, "null pointer");
+    DOP_REQUIRE((uintptr_t)logits % 16 == 0, "logits must be 16-byte aligned");
+    auto* m = reinterpret_cast<dop::Model*>(m_);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (m->prec == DOP_F32) m->forward<float>((const float*)params, tokens, logits, s);
+    else m->forward<dop::bf16>((const dop::bf16*)params, tokens, logits, s);
+  })
+}
+
+int dop_model_backward(dop_model* m_, const void* params, const int64_t* tokens,
+                       int grad_precision, const void* dlogits, float* dparams, void* stream) {
+  DOP_MODEL_GUARD({
+    DOP_REQUIRE(m_ && params && tokens && dlogits && dparams, "null pointer");
+    DOP_REQUIRE((uintptr_t)dlogits % 16 == 0, "dlogits must be 16-byte aligned");
+    auto* m = reinterpret_cast<dop::Model*>(m_);
+    DOP_REQUIRE(grad_precision == DOP_F32 || (grad_precision == DOP_BF16 && m->prec == DOP_BF16),
+                "dlogits must be fp32, or bf16 for a bf16 model");
+    if (!m->have_tape) throw dop::Error(DOP_E_STATE, "backward called before forward");
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (m->prec == DOP_F32)
+      m->backward<float>((const float*)params, tokens, dlogits, grad_precision, dparams, s);
+    else
+      m->backward<dop::bf16>((const dop::bf16*)params, tokens, dlogits, grad_precision, dparams, s);
   })
 }
 

@@ -70,6 +70,7 @@ class LinC(C.Structure):
 # (name, restype, argtypes) of every symbol include/dop.h declares.
 _P = C.c_void_p
 _I64 = C.c_int64
+_D = C.c_double
 SIGNATURES = [
     ("dop_last_error", C.c_char_p, []),
     ("dop_version", C.c_char_p, []),
@@ -97,6 +98,8 @@ SIGNATURES = [
     ("dop_model_create", C.c_int, [C.POINTER(MixtralCfg), _I64, _I64, C.c_int, C.POINTER(_P)]),
     ("dop_model_destroy", C.c_int, [_P]),
     ("dop_model_forward_backward", C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P]),
+    ("dop_model_forward", C.c_int, [_P, _P, _P, _P, _P]),
+    ("dop_model_backward", C.c_int, [_P, _P, _P, C.c_int, _P, _P, _P]),
     ("dop_model_parameter_count", _I64, [_P]),
     ("dop_lens_from_block", C.c_int, [_P, _P, _P, C.POINTER(_P)]),
     ("dop_compose", C.c_int, [_P, _P, C.POINTER(_P)]),
@@ -124,6 +127,16 @@ SIGNATURES = [
                                    _P, _P, _P, _P, _P, _P, _P]),
     ("dop_gqa_backward_f32_noalloc", C.c_int, [_I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P,
                                                _P, _P, _P, _P, _P, _P, _P]),
+    ("dop_token_logp", C.c_int, [_I64, _I64, C.c_int, _P, _I64, _P, _P, _D, _P, _P, _P]),
+    ("dop_token_logp_backward", C.c_int, [_I64, _I64, C.c_int, _P, _I64, _P, _P, _P, _D, C.c_int,
+                                          _P, _I64, _P]),
+    ("dop_policy_loss_grad", C.c_int, [_I64, _I64, C.c_int, _P, _I64, _P, _P, _P, _P, _P, _D, _D,
+                                       _D, _D, _D, _P, _P, _P, C.c_int, _P, _I64, _P]),
+    ("dop_preference_loss_grad", C.c_int, [_I64, _I64, C.c_int, _P, _I64, _P, _I64, _P, _P, _P,
+                                           _D, _D, _D, C.c_int, _D, _P, _P, _P, _P, _P, _P,
+                                           C.c_int, _P, _I64, _P]),
+    ("dop_distill_loss_grad", C.c_int, [_I64, _I64, C.c_int, _P, _I64, _I64, _P, _P, _P, _P, _D,
+                                        _D, _P, _P, C.c_int, _P, _I64, _P]),
     ("dop_f32_to_bf16", C.c_int, [_P, _P, _I64, _P]),
     ("dop_sgd_step", C.c_int, [_P, _P, _I64, C.c_float, _P]),
     ("dop_derive_links", C.c_int, [_P, _I64, _P, _I64, C.POINTER(_I64)]),

@@ -324,6 +324,36 @@ class Model:
                                                stream_ptr(stream)))
         return LossGrad(loss, grad, logits)
 
+    def forward(self, params, tokens, logits=None, stream=None):
+        """The get: logits fp32 [batch*seq, vocab]; the residual stays in the
+        handle for `backward`.  stream None is the current stream."""
+        import torch
+        stream = stream or torch.cuda.current_stream(params.device)
+        if logits is None:
+            logits = torch.empty(self.batch * self.seq, self.cfg.vocab, dtype=torch.float32,
+                                 device=params.device)
+        check(lib().dop_model_forward(self._h, ptr(params), ptr(tokens), ptr(logits),
+                                      stream_ptr(stream)))
+        return logits
+
+    def backward(self, params, tokens, dlogits, grad=None, stream=None):
+        """The put: the parameter adjoint of the last forward's logits from
+        their cotangent dlogits [batch*seq, vocab] (contiguous; fp32, or bf16
+        for a bf16 model), e.g. one of `dop.losses`.  `grad` is overwritten.
+        stream None is the current stream."""
+        import torch
+        stream = stream or torch.cuda.current_stream(params.device)
+        if (dlogits.shape != (self.batch * self.seq, self.cfg.vocab) or not dlogits.is_contiguous()
+                or dlogits.dtype not in (torch.float32, torch.bfloat16)):
+            raise _lib.DopError(-1, "invalid argument: dlogits must be a contiguous fp32 or bf16 "
+                                    "tensor [batch*seq, vocab]")
+        if grad is None:
+            grad = torch.empty(self.n_params, dtype=torch.float32, device=params.device)
+        prec = DOP_F32 if dlogits.dtype is torch.float32 else DOP_BF16
+        check(lib().dop_model_backward(self._h, ptr(params), ptr(tokens), prec, ptr(dlogits),
+                                       ptr(grad), stream_ptr(stream)))
+        return grad
+
 
 def forward_backward(cfg: MixtralConfig, params, tokens, targets, batch: int, seq: int,
                      precision: int = DOP_F32) -> LossGrad:

@@ -190,6 +190,19 @@ int dop_model_forward_backward(dop_model* m, const void* params,
                                const int64_t* tokens, const int64_t* targets,
                                float* loss, float* dparams, float* logits,
                                void* stream);
+/* The model's get and put as calls of their own, for an objective of the
+ * caller's (the objectives over logits below).  dop_model_forward writes the
+ * logits (fp32 [batch*seq, vocab]) and keeps its residual in the handle;
+ * dop_model_backward takes the residual of the last forward (of either kind),
+ * the same params and tokens, and dlogits [batch*seq, vocab] contiguous in
+ * grad_precision (DOP_F32, or DOP_BF16 for a bf16 model: what its head's
+ * gradient GEMMs read), and OVERWRITES dparams.  Both matrices are 16-byte
+ * aligned.  dop_model_forward_backward is the two calls with the
+ * cross-entropy between them. */
+int dop_model_forward(dop_model* m, const void* params, const int64_t* tokens,
+                      float* logits, void* stream);
+int dop_model_backward(dop_model* m, const void* params, const int64_t* tokens,
+                       int grad_precision, const void* dlogits, float* dparams, void* stream);
 int64_t dop_model_parameter_count(const dop_model* m);
 
 /* ------------------------------------------------------- lens composition
@@ -295,6 +308,89 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
                                  const float* q, const float* k, const float* v,
                                  const float* o, const float* dout, const float* lse,
                                  float* dq, float* dk, float* dv, void* stream);
+
+/* ------------------------------------------- objectives over a model's logits
+ * What the model lens is trained on after next-token cross-entropy
+ * (src/mixtral.rs:966-991): each call reads logits z [rows, vocab] and writes
+ * the loss and its adjoint dlogits, which dop_model_backward takes.  They have
+ * no counterpart in the crate.  Conventions of all of them:
+ *
+ *   - x = z / temperature, lse = log sum exp x, p = exp(x - lse).  Row r starts
+ *     at logits + r * ld elements (ld >= vocab).  `precision` is the logits'
+ *     type; dlogits has `grad_precision`: DOP_BF16, or DOP_F32 for fp32 logits.
+ *     dlogits may be the logits' own memory when type and stride are the same
+ *     (ldd == ld); any other overlap is refused.  dlogits is ASSIGNED, all of
+ *     its rows x vocab elements and nothing between the rows; dlogits NULL
+ *     computes the loss alone (not in dop_token_logp_backward).
+ *   - Sums and statistics are fp32 or wider; a row's scalars, and the sums
+ *     over rows, are fp64 in a fixed order, so that equal inputs give equal
+ *     bytes.  No call allocates, synchronises or keeps anything: all of them
+ *     can be captured in a graph, and calls on different streams share nothing.
+ *   - weight [rows] (NULL: 1) is a mask and a factor.  A row whose weight is 0,
+ *     or whose token lies outside [0, vocab), is skipped: its logits are not
+ *     read, its outputs and its row of dlogits are 0.
+ *   - A logit of -inf is an entry of probability 0.  A row that is not skipped
+ *     and has no finite logit, or a NaN or +inf among them, gives NaN.
+ *   - loss is one float: scale times the sum over rows (pairs); 0 rows: 0.
+ *
+ * Token log-probabilities: logp[r] = x[tokens[r]] - lse[r]; both are 0 for a
+ * skipped row.  Backward: dlogits = dlogp / temperature ([v = token] - p), from
+ * the lse of the forward; rows with dlogp 0 or a token outside [0, vocab) are
+ * skipped. */
+int dop_token_logp(int64_t rows, int64_t vocab, int precision, const void* logits, int64_t ld,
+                   const int64_t* tokens, const float* weight, double temperature,
+                   float* logp, float* lse, void* stream);
+int dop_token_logp_backward(int64_t rows, int64_t vocab, int precision, const void* logits,
+                            int64_t ld, const int64_t* tokens, const float* lse,
+                            const float* dlogp, double temperature, int grad_precision,
+                            void* dlogits, int64_t ldd, void* stream);
+/* The clipped policy loss with a KL term: with ratio = exp(logp - old_logp),
+ * gap = ref_logp - logp and advantage A,
+ *   row_loss = weight (-min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *                      + kl_coef (exp(gap) - gap - 1)).
+ * ref_logp may be NULL when kl_coef is 0.  A ratio on the clip's border counts
+ * as inside.  logp [rows] receives the current log-probabilities. */
+int dop_policy_loss_grad(int64_t rows, int64_t vocab, int precision, const void* logits,
+                         int64_t ld, const int64_t* tokens, const float* old_logp,
+                         const float* advantage, const float* ref_logp, const float* weight,
+                         double temperature, double clip_low, double clip_high, double kl_coef,
+                         double scale, float* loss, float* row_loss, float* logp,
+                         int grad_precision, void* dlogits, int64_t ldd, void* stream);
+/* The preference loss over `pairs` pairs of sequences packed in the rows.
+ * seq_off is a HOST array of 2 pairs + 1 row offsets, not decreasing, within
+ * [0, rows]: pair i's chosen sequence is rows [seq_off[2i], seq_off[2i+1]),
+ * its rejected one [seq_off[2i+1], seq_off[2i+2]); rows of no sequence are
+ * skipped.  S = sum of weight (logp - ref_logp) over a sequence (ref_logp NULL:
+ * 0), divided by the sum of its weights with length_normalize (0 for none);
+ *   margin = beta (S_chosen - S_rejected),
+ *   pair_loss = -(1 - label_smoothing) log sigma(margin)
+ *               - label_smoothing log sigma(-margin).
+ * logp, lse and dlogp [rows] receive the log-probabilities, their log-sum-exp
+ * and the loss's adjoint with respect to logp. */
+int dop_preference_loss_grad(int64_t rows, int64_t vocab, int precision, const void* logits,
+                             int64_t ld, const int64_t* tokens, int64_t pairs,
+                             const int64_t* seq_off, const float* ref_logp, const float* weight,
+                             double temperature, double beta, double label_smoothing,
+                             int length_normalize, double scale, float* loss, float* pair_loss,
+                             float* margin, float* logp, float* lse, float* dlogp,
+                             int grad_precision, void* dlogits, int64_t ldd, void* stream);
+/* Distillation from a teacher's top logits.  top_index [rows, top_k] names
+ * vocabulary entries (one outside [0, vocab) is absent; an entry named twice
+ * has the sum of its probabilities), top_logit [rows, top_k] holds the
+ * teacher's logits there, -inf for probability 0; top_k <= 1024.  With
+ * teacher_lse NULL, q is the softmax of top_logit / temperature over the
+ * row's entries:
+ *   row_loss = weight temperature^2 sum_k q_k (log q_k - log p_{top_index[k]}).
+ * With teacher_lse [rows], the log-sum-exp of the teacher's whole row over
+ * temperature, q_k = exp(top_logit_k / temperature - teacher_lse) and what
+ * both distributions hold outside the row's entries is one more class:
+ * q_r = max(0, 1 - sum q), p_r = the sum of p there (none when the entries
+ * are the whole vocabulary).  A row without entries has loss 0. */
+int dop_distill_loss_grad(int64_t rows, int64_t vocab, int precision, const void* logits,
+                          int64_t ld, int64_t top_k, const int32_t* top_index,
+                          const float* top_logit, const float* teacher_lse, const float* weight,
+                          double temperature, double scale, float* loss, float* row_loss,
+                          int grad_precision, void* dlogits, int64_t ldd, void* stream);
 
 /* ------------------------------------------------- failure detection
  * Every wait a libdop kernel makes on another agent is bounded: mbarrier
