@@ -17,6 +17,7 @@
 // writes the adjoint.
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "../../include/dop.h"
 #include "kernels.cuh"
@@ -31,6 +32,10 @@ enum RowOp : int { kLogp = 0, kLogpBwd = 1, kPolicy = 2, kDistill = 3 };
 
 constexpr int kRowThreads = 256;
 constexpr int kMaxTeacherK = 1024;
+constexpr int kMaxCluster = 8;
+// Shared memory of a CTA's pieces: three CTAs fit an SM up to kStageBytes,
+// one up to kStageBytesMost.
+constexpr int64_t kStageBytes = 72 * 1024, kStageBytesMost = 200 * 1024;
 constexpr double kLog2e = 1.4426950408889634;
 
 struct RowArgs {
@@ -43,6 +48,8 @@ struct RowArgs {
   const float* weight;  // null: 1
   double inv_tau;
   float c;       // log2(e) / tau
+  int cluster;      // CTAs per row
+  int stage_bytes;  // of shared memory for a CTA's pieces
   double scale;  // of the loss and the adjoint
   float* logp;
   float* logp_lo;  // null, or what logp's rounding to fp32 left out
@@ -93,25 +100,109 @@ __device__ double block_sum_d(double v, double* red) {
   return t;
 }
 
-// One CTA per row.
+// ---- a row in shared memory
+// A row is cut into 16-byte pieces at 16-byte borders of its address, so a
+// row may start and end inside a piece; the cluster's CTAs hold consecutive
+// runs of pieces, one CTA the whole row when it fits.  A thread copies pieces
+// tid, tid + 256, ... and is the one that reads them back for the maximum and
+// sum, so that pass needs no barrier.  What a piece holds beyond the row is -inf.
+__device__ __forceinline__ void copy_piece(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Wait until at most `n` of this thread's copy groups are under way.
+__device__ __forceinline__ void copy_wait(int n) {
+  switch (n) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
+    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
+  }
+}
+__device__ __forceinline__ float2 bf16x2(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+// The elements of a piece as pairs.
+__device__ __forceinline__ void unpack(uint4 u, float2* x, const float*) {
+  x[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+  x[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+}
+__device__ __forceinline__ void unpack(uint4 u, float2* x, const bf16*) {
+  x[0] = bf16x2(u.x);
+  x[1] = bf16x2(u.y);
+  x[2] = bf16x2(u.z);
+  x[3] = bf16x2(u.w);
+}
+__device__ __forceinline__ uint32_t minus_inf_word(const float*) { return 0xff800000u; }
+__device__ __forceinline__ uint32_t minus_inf_word(const bf16*) { return 0xff80ff80u; }
+__device__ __forceinline__ void store_unit(float* p, const float* v) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store_unit(bf16* p, const float* v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(tc::pack_bf16(v[0], v[1]), tc::pack_bf16(v[2], v[3]),
+                                            tc::pack_bf16(v[4], v[5]), tc::pack_bf16(v[6], v[7]));
+}
+
+// What the CTAs of a cluster tell one another of their part of the row.
+struct alignas(16) Part {
+  MaxSum rest;    // entries not listed by the teacher (all, elsewhere)
+  MaxSum listed;  // listed entries, each vocabulary entry once
+  float count;    // of the listed entries
+};
+static_assert(sizeof(Part) == 32, "a Part is written to a peer as 16 + 4 bytes");
+
+// A cluster of `nctarank` CTAs per row.
 template <RowOp OP, typename TI, typename TO>
-__global__ void __launch_bounds__(kRowThreads) k_vocab_row(const RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
+  constexpr int EI = 16 / (int)sizeof(TI), EO = 16 / (int)sizeof(TO);
+  constexpr int NT = kRowThreads, NW = NT / 32, U = 4;
   extern __shared__ __align__(16) uint8_t dyn[];
-  __shared__ MaxSum s_ms[kRowThreads / 32];
-  __shared__ double s_red[kRowThreads / 32];
-  __shared__ float s_coef[2];
-  const int64_t row = blockIdx.x;
+  __shared__ Part s_warp[NW];
+  __shared__ Part s_peer[kMaxCluster];
+  __shared__ double s_red[2][NW];
+  __shared__ float s_coef[4];
+  __shared__ int s_twice;
+  const int C = a.cluster, rank = (int)blockIdx.x % C, tid = threadIdx.x, lane = tid & 31;
+  const int64_t row = blockIdx.x / C;
   const TI* z = (const TI*)a.z + row * a.ld;
   TO* dz = a.dz ? (TO*)a.dz + row * a.ldd : nullptr;
-  const int64_t V = a.V;
+  const int V = (int)a.V;
+  // this CTA's pieces [p0, p1) and elements [e_lo, e_hi)
+  const int ph = (int)((uintptr_t)z & 15) / (int)sizeof(TI);
+  const int64_t pieces = ((int64_t)ph + V + EI - 1) / EI;
+  const int p0 = (int)(pieces * rank / C), np = (int)(pieces * (rank + 1) / C) - p0;
+  const int e_org = (int)((int64_t)p0 * EI - ph);  // the row's element at image element 0
+  const int e_lo = max(0, e_org), e_hi = (int)min((int64_t)V, (int64_t)e_org + (int64_t)np * EI);
+  // units of 16 bytes of dz: whole ones [u0, u1), the rest of the elements ahead and behind
+  const int dph = dz ? (int)((uintptr_t)dz & 15) / (int)sizeof(TO) : 0;
+  const int64_t u0 = ((int64_t)dph + e_lo + EO - 1) / EO, u1 = ((int64_t)dph + e_hi) / EO;
+
   const float w = a.weight ? a.weight[row] : 1.f;
-  const int64_t token = OP == kDistill ? 0 : a.tokens[row];
-  bool skip = w == 0.f || token < 0 || token >= V;
+  const int64_t token = OP == kDistill ? -1 : a.tokens[row];
+  bool skip = w == 0.f || (OP != kDistill && (token < 0 || token >= V));
   if (OP == kLogpBwd && a.dlogp[row] == 0.f) skip = true;
+
+  // elements of the units that are not whole: f(element)
+  auto ragged = [&](auto f) {
+    if (u0 >= u1) {
+      for (int e = e_lo + tid; e < e_hi; e += NT) f(e);
+    } else {
+      const int ahead = (int)(u0 * EO - dph) - e_lo, behind0 = (int)(u1 * EO - dph);
+      if (tid < ahead) f(e_lo + tid);
+      if (tid >= 32 && tid - 32 < e_hi - behind0) f(behind0 + tid - 32);
+    }
+  };
   if (skip) {
-    if (dz)
-      for (int64_t v = threadIdx.x; v < V; v += kRowThreads) st(&dz[v], 0.f);
-    if (threadIdx.x == 0) {
+    if (dz) {
+      const float zero[EO] = {};
+      for (int64_t u = u0 + tid; u < u1; u += NT) store_unit(dz + (u * EO - dph), zero);
+      ragged([&](int e) { st(&dz[e], 0.f); });
+    }
+    if (tid == 0 && rank == 0) {
       if (OP != kLogpBwd && OP != kDistill && a.logp) a.logp[row] = 0.f;
       if (OP == kLogp && a.lse) a.lse[row] = 0.f;
       if (OP == kLogp && a.logp_lo) a.logp_lo[row] = 0.f;
@@ -119,70 +210,191 @@ __global__ void __launch_bounds__(kRowThreads) k_vocab_row(const RowArgs a) {
     }
     return;
   }
-  const float za = OP == kDistill ? 0.f : ld(&z[token]);
+  // every CTA of the cluster has started once this barrier is through: its
+  // shared memory may be written to
+  if (OP != kLogpBwd && C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
-  // ---- the teacher's entries: q, the student's logit, and which are a
-  // vocabulary entry's first
-  int32_t* t_idx = (int32_t*)dyn;
-  float* t_q = (float*)(t_idx + a.K);
-  float* t_z = t_q + a.K;
-  uint32_t* bits = (uint32_t*)(t_z + a.K);
+  // ---- copy this CTA's pieces
+  const uint32_t img = tc::smem_u32(dyn);
+  TI* image = (TI*)dyn;
+  const TI* src = z + e_org;
+  const int rounds = (np + U * NT - 1) / (U * NT);
+  for (int r = 0; r < rounds; ++r) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = tid + (r * U + j) * NT;
+      if (i >= np) continue;
+      const int e = e_org + i * EI;
+      if (e >= 0 && e <= V - EI) {
+        copy_piece(img + i * 16, src + (int64_t)i * EI);
+      } else {
+        for (int k = 0; k < EI; ++k)
+          image[i * EI + k] = e + k >= 0 && e + k < V ? z[e + k] : (TI)-INFINITY;
+      }
+    }
+    copy_commit();
+  }
+  const float za = OP == kDistill || OP == kLogpBwd ? 0.f : ld(&z[token]);
+
+  // ---- the teacher's entries while the copies run: q, the student's logit
+  int32_t* t_idx = (int32_t*)(dyn + a.stage_bytes);
+  float* t_q = (float*)(t_idx + a.K);  // q
+  float* t_z = t_q + a.K;              // the student's logit
+  float* t_g = t_z + a.K;              // this CTA's first ones: sum of q of the entry; else -1
   double q_sum = 0.0, q_logq = 0.0, q_rest = 0.0;
   if (OP == kDistill) {
-    for (int64_t i = threadIdx.x; i < (V + 31) / 32; i += kRowThreads) bits[i] = 0;
     const float* y = a.top_logit + row * a.K;
     MaxSum t = {-INFINITY, 0.f};
-    for (int k = threadIdx.x; k < a.K; k += kRowThreads) {
+    for (int k = tid; k < a.K; k += NT) {
       const int32_t i = a.top_index[row * a.K + k];
       const bool in = i >= 0 && i < V;
+      const float yk = in ? y[k] : -INFINITY;
       t_idx[k] = in ? i : -1;
       t_z[k] = in ? ld(&z[i]) : 0.f;
-      t_q[k] = in ? y[k] : -INFINITY;
-      if (in) t = join(t, {y[k], 1.f}, a.c);
+      t_q[k] = yk;
+      if (in) t = join(t, {yk, 1.f}, a.c);
     }
-    t = warp_join(t, a.c);
-    if ((threadIdx.x & 31) == 0) s_ms[threadIdx.x >> 5] = t;
-    __syncthreads();
-    t = s_ms[0];
-    for (int i = 1; i < kRowThreads / 32; ++i) t = join(t, s_ms[i], a.c);
-    const double tl = a.teacher_lse ? (double)a.teacher_lse[row]
-                                    : (double)base_of(t.m) * a.inv_tau + log((double)t.s);
+    if (tid == 0) s_twice = 0;
+    double tl;
+    if (a.teacher_lse) {
+      tl = (double)a.teacher_lse[row];
+    } else {
+      t = warp_join(t, a.c);
+      if (lane == 0) s_warp[tid >> 5].rest = t;
+      __syncthreads();
+      t = s_warp[0].rest;
+      for (int i = 1; i < NW; ++i) t = join(t, s_warp[i].rest, a.c);
+      tl = (double)base_of(t.m) * a.inv_tau + log((double)t.s);
+    }
     double qs = 0.0, ql = 0.0;
-    for (int k = threadIdx.x; k < a.K; k += kRowThreads) {
+    for (int k = tid; k < a.K; k += NT) {
       const double lq = (double)t_q[k] * a.inv_tau - tl;
       const double q = t_idx[k] < 0 || t_q[k] == -INFINITY ? 0.0 : exp(lq);
       t_q[k] = (float)q;
       qs += q;
       if (q > 0.0) ql += q * lq;
-      if (t_idx[k] >= 0) atomicOr(&bits[t_idx[k] >> 5], 1u << (t_idx[k] & 31));
     }
-    q_sum = block_sum_d(qs, s_red);
-    q_logq = block_sum_d(ql, s_red);
+    qs = warp_sum_d(qs);
+    ql = warp_sum_d(ql);
+    if (lane == 0) {
+      s_red[0][tid >> 5] = qs;
+      s_red[1][tid >> 5] = ql;
+    }
+    // ---- listed entries leave the image: -inf, and each counts once.  A word
+    // of all ones marks an entry; one found marked is named twice (or was that
+    // NaN), and then the entries are compared one by one.
+    copy_wait(0);
+    __syncthreads();
+    for (int i = 0; i < NW; ++i) {
+      q_sum += s_red[0][i];
+      q_logq += s_red[1][i];
+    }
     q_rest = a.teacher_lse ? fmax(0.0, 1.0 - q_sum) : 0.0;
+    auto here = [&](int k) { return t_idx[k] >= e_lo && t_idx[k] < e_hi; };
+    uint32_t* words = (uint32_t*)dyn;
+    for (int k = tid; k < a.K; k += NT) {
+      t_g[k] = here(k) ? t_q[k] : -1.f;
+      if (!here(k)) continue;
+      const uint32_t at = (uint32_t)(t_idx[k] - e_org) * sizeof(TI);
+      const uint32_t ones = (sizeof(TI) == 4 ? 0xffffffffu : 0xffffu) << (8 * (at & 3));
+      if ((atomicOr(&words[at >> 2], ones) & ones) == ones) s_twice = 1;
+    }
+    __syncthreads();
+    for (int k = tid; k < a.K; k += NT) {
+      if (!here(k)) continue;
+      image[t_idx[k] - e_org] = (TI)-INFINITY;
+      if (s_twice) {
+        double g = 0.0;
+        bool first = true;
+        for (int j = 0; j < a.K; ++j)
+          if (t_idx[j] == t_idx[k]) {
+            if (j < k) first = false;
+            g += (double)t_q[j];
+          }
+        t_g[k] = first ? (float)g : -1.f;
+      }
+    }
+    __syncthreads();
   }
 
   // ---- maximum and sum
-  MaxSum r = {-INFINITY, 0.f};
+  Part part = {{-INFINITY, 0.f}, {-INFINITY, 0.f}, 0.f};
   if (OP != kLogpBwd) {
-    for (int64_t v = threadIdx.x; v < V; v += kRowThreads) {
-      const float x = ld(&z[v]);
-      if (OP == kDistill && (bits[v >> 5] >> (v & 31) & 1u)) continue;
-      if (x > r.m) {
-        r.s *= tc::fast_exp2((r.m - x) * a.c);
-        r.m = x;
+    float m = -INFINITY;
+    float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
+    const float2 c2 = make_float2(a.c, a.c);
+    const uint32_t none = minus_inf_word((const TI*)nullptr);
+    for (int r = 0; r < rounds; ++r) {
+      if (OP != kDistill) copy_wait(rounds - 1 - r);
+      float2 x[U][EI / 2];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = tid + (r * U + j) * NT;
+        const uint4 u = i < np ? ((const uint4*)dyn)[i] : make_uint4(none, none, none, none);
+        unpack(u, x[j], (const TI*)nullptr);
+#pragma unroll
+        for (int k = 0; k < EI / 2; ++k) mx = tc::fmax3(mx, x[j][k].x, x[j][k].y);
       }
-      r.s += tc::fast_exp2((x - base_of(r.m)) * a.c);
+      if (mx > m) {
+        const float k = tc::fast_exp2((m - mx) * a.c);
+        s0 = tc::fmul2(s0, make_float2(k, k));
+        s1 = tc::fmul2(s1, make_float2(k, k));
+        m = mx;
+      }
+      const float2 nb = make_float2(-base_of(m), -base_of(m));
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int k = 0; k < EI / 2; ++k) {
+          const float2 t = tc::fmul2(tc::fadd2(x[j][k], nb), c2);
+          const float2 e = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
+          if (k & 1) s1 = tc::fadd2(s1, e);
+          else s0 = tc::fadd2(s0, e);
+        }
     }
-    r = warp_join(r, a.c);
+    part.rest = warp_join({m, (s0.x + s0.y) + (s1.x + s1.y)}, a.c);
+    if (OP == kDistill) {
+      MaxSum in = {-INFINITY, 0.f};
+      float n = 0.f;
+      for (int k = tid; k < a.K; k += NT)
+        if (!(t_g[k] < 0.f)) {
+          in = join(in, {t_z[k], t_z[k] == -INFINITY ? 0.f : 1.f}, a.c);
+          n += 1.f;
+        }
+      part.listed = warp_join(in, a.c);
+      part.count = warp_sum(n);
+    }
+    if (lane == 0) s_warp[tid >> 5] = part;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_ms[threadIdx.x >> 5] = r;
-    __syncthreads();
-    r = s_ms[0];
-    for (int i = 1; i < kRowThreads / 32; ++i) r = join(r, s_ms[i], a.c);
+    auto add = [&](Part& to, const Part& p) {
+      to.rest = join(to.rest, p.rest, a.c);
+      if (OP == kDistill) {
+        to.listed = join(to.listed, p.listed, a.c);
+        to.count += p.count;
+      }
+    };
+    part = s_warp[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) add(part, s_warp[i]);
+    if (C > 1) {
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+      if (tid < C) {
+        const uint32_t to = tc::mapa_shared(tc::smem_u32(&s_peer[rank]), (uint32_t)tid);
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to),
+                     "f"(part.rest.m), "f"(part.rest.s), "f"(part.listed.m), "f"(part.listed.s)
+                     : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 16), "f"(part.count) : "memory");
+      }
+      tc::cluster_sync();
+      part = s_peer[0];
+      for (int i = 1; i < C; ++i) add(part, s_peer[i]);
+    }
   }
+  const MaxSum r = part.rest;
 
   // ---- the row's scalars: dz = c_out 2^((f z - b) c) + corrections
-  float c_in = 0.f, b_in = 0.f, c_out = 0.f, hot = 0.f, b = 0.f, f = 1.f, c = a.c;
+  float c_in = 0.f, b_in = 0.f, c_out = 0.f, hot = 0.f, b = base_of(r.m), f = 1.f, c = a.c;
   if (OP == kLogpBwd) {
     hot = (float)((double)a.dlogp[row] * a.inv_tau);
     c_out = -hot;
@@ -190,12 +402,14 @@ __global__ void __launch_bounds__(kRowThreads) k_vocab_row(const RowArgs a) {
     b = a.lse[row];
     c = (float)kLog2e;
   } else if (OP != kDistill) {
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
       const double ls = log((double)r.s);
-      const double logp = ((double)za - (double)base_of(r.m)) * a.inv_tau - ls;
-      if (a.logp) a.logp[row] = (float)logp;
-      if (OP == kLogp && a.logp_lo) a.logp_lo[row] = (float)(logp - (double)(float)logp);
-      if (OP == kLogp && a.lse) a.lse[row] = (float)((double)base_of(r.m) * a.inv_tau + ls);
+      const double logp = ((double)za - (double)b) * a.inv_tau - ls;
+      if (rank == 0) {
+        if (a.logp) a.logp[row] = (float)logp;
+        if (OP == kLogp && a.logp_lo) a.logp_lo[row] = (float)(logp - (double)(float)logp);
+        if (OP == kLogp && a.lse) a.lse[row] = (float)((double)b * a.inv_tau + ls);
+      }
       if (OP == kPolicy) {
         const double A = a.advantage[row], ratio = exp(logp - (double)a.old_logp[row]);
         const double lo = 1.0 - a.clip_low, hi = 1.0 + a.clip_high;
@@ -207,46 +421,35 @@ __global__ void __launch_bounds__(kRowThreads) k_vocab_row(const RowArgs a) {
           l += a.kl_coef * (e - gap);
           d -= a.kl_coef * e;
         }
-        a.row_loss[row] = (float)((double)w * l);
+        if (rank == 0) a.row_loss[row] = (float)((double)w * l);
         const double g = a.scale * (double)w * d * a.inv_tau;
         s_coef[0] = (float)g;
         s_coef[1] = (float)(-g / (double)r.s);
       }
     }
+    if (OP == kLogp || !dz) return;
     __syncthreads();
     hot = s_coef[0];
     c_out = s_coef[1];
   } else {
-    // the listed entries join the sum: each vocabulary entry once
-    MaxSum in = {-INFINITY, 0.f};
-    double listed = 0.0;
-    for (int k = threadIdx.x; k < a.K; k += kRowThreads) {
-      bool first = t_idx[k] >= 0;
-      for (int j = 0; j < k && first; ++j) first = t_idx[j] != t_idx[k];
-      if (first) in = join(in, {t_z[k], t_z[k] == -INFINITY ? 0.f : 1.f}, a.c);
-      if (first) listed += 1.0;
-    }
+    const MaxSum all = join(r, part.listed, a.c);
     // without an entry outside the list there is no class for the rest
-    if (block_sum_d(listed, s_red) == (double)V) q_rest = 0.0;
-    in = warp_join(in, a.c);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s_ms[threadIdx.x >> 5] = in;
-    __syncthreads();
-    in = s_ms[0];
-    for (int i = 1; i < kRowThreads / 32; ++i) in = join(in, s_ms[i], a.c);
-    const MaxSum all = join(r, in, a.c);
+    if (part.count == (float)V) q_rest = 0.0;
     const double ls = log((double)all.s), mx = (double)base_of(all.m) * a.inv_tau;
     double cross = 0.0;
-    for (int k = threadIdx.x; k < a.K; k += kRowThreads)
+    for (int k = tid; k < a.K; k += NT)
       if (t_q[k] != 0.f) cross += (double)t_q[k] * ((double)t_z[k] * a.inv_tau - mx - ls);
-    cross = block_sum_d(cross, s_red);
-    if (threadIdx.x == 0) {
-      double l = q_logq - cross;
-      if (q_rest > 0.0)
-        l += q_rest * (log(q_rest) -
-                       ((double)base_of(r.m) * a.inv_tau + log((double)r.s) - mx - ls));
-      a.row_loss[row] = (float)((double)w * l / (a.inv_tau * a.inv_tau));
+    if (rank == 0) {
+      cross = block_sum_d(cross, s_red[0]);
+      if (tid == 0) {
+        double l = q_logq - cross;
+        if (q_rest > 0.0)
+          l += q_rest *
+               (log(q_rest) - ((double)b * a.inv_tau + log((double)r.s) - mx - ls));
+        a.row_loss[row] = (float)((double)w * l / (a.inv_tau * a.inv_tau));
+      }
     }
+    if (!dz) return;
     const double g = a.scale * (double)w / a.inv_tau;
     const double Q = q_sum + q_rest;
     c_in = (float)(g * Q / (double)all.s);
@@ -255,29 +458,61 @@ __global__ void __launch_bounds__(kRowThreads) k_vocab_row(const RowArgs a) {
     // mass outside may be too small to be held relative to the row's largest
     // (none at all: an infinite loss, and entries of probability 0)
     c_out = r.s == 0.f ? 0.f
-                       : (float)(g * (Q * (double)tc::fast_exp2((base_of(r.m) - b_in) * a.c) /
-                                          (double)all.s -
+                       : (float)(g * (Q * (double)tc::fast_exp2((b - b_in) * a.c) / (double)all.s -
                                       (q_rest > 0.0 ? q_rest / (double)r.s : 0.0)));
     hot = (float)g;
   }
 
-  // ---- the adjoint
-  if (!dz) return;
-  if (OP != kLogpBwd) b = base_of(r.m);
-  for (int64_t v = threadIdx.x; v < V; v += kRowThreads) {
-    const float x = ld(&z[v]);
-    float d = c_out * tc::fast_exp2(fmaf(x, f, -b) * c);
-    if (OP == kDistill) {
-      if (bits[v >> 5] >> (v & 31) & 1u) {
-        double q = 0.0;
-        for (int k = 0; k < a.K; ++k)
-          if (t_idx[k] == v) q += t_q[k];
-        d = c_in * tc::fast_exp2((x - b_in) * c) - hot * (float)q;
-      }
-    } else if (v == token) {
-      d += hot;
+  // ---- the adjoint, in 16-byte units of dz; an image whose pieces do not
+  // line up with them is read element by element
+  if (OP == kLogpBwd) {
+    copy_wait(0);
+    __syncthreads();
+  }
+  const float2 f2 = make_float2(f, f), nb = make_float2(-b, -b), c2 = make_float2(c, c);
+  auto value = [&](float x) { return c_out * tc::fast_exp2(fmaf(x, f, -b) * c); };
+  const bool aligned = ((int)(u0 * EO - dph) - e_org) % EI == 0;
+  auto unit = [&](int64_t u, auto lined_up) {
+    const int e0 = (int)(u * EO - dph), at = e0 - e_org;
+    float2 x[EO / 2];
+    float v[EO];
+    if constexpr (decltype(lined_up)::value) {
+#pragma unroll
+      for (int q = 0; q < EO / EI; ++q)
+        unpack(((const uint4*)dyn)[at / EI + q], &x[q * (EI / 2)], (const TI*)nullptr);
+    } else {
+#pragma unroll
+      for (int k = 0; k < EO / 2; ++k) x[k] = make_float2(ld(&image[at + 2 * k]), ld(&image[at + 2 * k + 1]));
     }
-    st(&dz[v], d);
+#pragma unroll
+    for (int k = 0; k < EO / 2; ++k) {
+      const float2 t = tc::fmul2(OP == kLogpBwd ? tc::ffma2(x[k], f2, nb) : tc::fadd2(x[k], nb), c2);
+      v[2 * k] = c_out * tc::fast_exp2(t.x);
+      v[2 * k + 1] = c_out * tc::fast_exp2(t.y);
+    }
+    if (OP != kDistill) {
+      const int64_t d = token - e0;
+      if (d >= 0 && d < EO) {
+#pragma unroll
+        for (int k = 0; k < EO; ++k)
+          if (d == k) v[k] += hot;
+      }
+    }
+    store_unit(dz + e0, v);
+  };
+  if (aligned) {
+#pragma unroll 2
+    for (int64_t u = u0 + tid; u < u1; u += NT) unit(u, std::true_type{});
+  } else {
+#pragma unroll 2
+    for (int64_t u = u0 + tid; u < u1; u += NT) unit(u, std::false_type{});
+  }
+  ragged([&](int e) { st(&dz[e], value(ld(&image[e - e_org])) + (e == token ? hot : 0.f)); });
+  if (OP == kDistill) {
+    __syncthreads();
+    for (int k = tid; k < a.K; k += NT)
+      if (!(t_g[k] < 0.f))
+        st(&dz[t_idx[k]], c_in * tc::fast_exp2((t_z[k] - b_in) * c) - hot * t_g[k]);
   }
 }
 
@@ -352,16 +587,37 @@ __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_co
 
 // ------------------------------------------------------------------- host
 template <RowOp OP>
-void launch_rows(const RowArgs& a, int64_t rows, int prec, int grad_prec, cudaStream_t s) {
+void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t s) {
   if (rows == 0) return;
-  DOP_REQUIRE(rows <= INT32_MAX, "rows");
-  const size_t smem = OP == kDistill ? 12 * (size_t)a.K + 4 * ((a.V + 31) / 32) : 0;
+  const int64_t bytes = a.V * (prec == DOP_BF16 ? 2 : 4) + 16;
+  int64_t C = ceil_div(bytes, kStageBytes);
+  if (C > kMaxCluster) {
+    C = kMaxCluster;
+    if (ceil_div(bytes, C) > kStageBytesMost - 16)
+      throw Error(DOP_E_UNSUPPORTED, "vocab (" + std::to_string(a.V) + ") is above " +
+                                         std::to_string(kMaxCluster * (kStageBytesMost - 32) /
+                                                        (prec == DOP_BF16 ? 2 : 4)));
+  }
+  if (rows * C > INT32_MAX) throw Error(DOP_E_UNSUPPORTED, "too many rows for this vocab");
+  a.cluster = (int)C;
+  a.stage_bytes = (int)round_up(ceil_div(bytes, C) + 16, 16);
+  const size_t smem = (size_t)a.stage_bytes + (OP == kDistill ? 16 * (size_t)a.K : 0);
   auto go = [&](auto ti, auto to) {
     auto kern = k_vocab_row<OP, decltype(ti), decltype(to)>;
-    if (smem > 48 * 1024)
-      DOP_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kern<<<(unsigned)rows, kRowThreads, smem, s>>>(a);
-    DOP_CHECK_CUDA(cudaGetLastError());
+    DOP_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)(kStageBytesMost + 16 * kMaxTeacherK)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * C));
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = C > 1 ? 1 : 0;
+    DOP_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   };
   if (prec == DOP_BF16) go(bf16{}, bf16{});
   else if (a.dz && grad_prec == DOP_BF16) go(0.f, bf16{});

@@ -322,9 +322,9 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  *     (ldd == ld); any other overlap is refused.  dlogits is ASSIGNED, all of
  *     its rows x vocab elements and nothing between the rows; dlogits NULL
  *     computes the loss alone (not in dop_token_logp_backward).
- *   - Sums and statistics are fp32 or wider; a row's scalars, and the sums
- *     over rows, are fp64 in a fixed order, so that equal inputs give equal
- *     bytes.  No call allocates, synchronises or keeps anything: all of them
+ *   - Sums and statistics are fp32 or wider, a row's scalars and the sums over
+ *     rows fp64, all in a fixed order: equal inputs in equally aligned rows
+ *     (address modulo 16) give equal bytes.  No call allocates, synchronises or keeps anything: all of them
  *     can be captured in a graph, and calls on different streams share nothing.
  *   - weight [rows] (NULL: 1) is a mask and a factor.  A row whose weight is 0,
  *     or whose token lies outside [0, vocab), is skipped: its logits are not

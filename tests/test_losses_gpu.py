@@ -558,9 +558,14 @@ def test_gradient_against_differences(cuda, which):
 
 # ------------------------------------- in place, streams, graphs, no memory
 def every(z, tokens, old, adv, ref, index, top, tlse, off, dlogits=None, stream=None):
-    """One call of each objective that writes dlogits; fresh copies of z."""
+    """One call of each objective that writes dlogits; with "own", into fresh
+    copies of z in z's own layout (a row's alignment sets its sum's order)."""
     def c():
-        return z.clone() if dlogits == "own" else z
+        if dlogits != "own":
+            return z
+        x = torch.empty(z.shape[0] * z.stride(0), dtype=z.dtype, device="cuda")
+        x = x.view(z.shape[0], z.stride(0))[:, :z.shape[1]]
+        return x.copy_(z)
 
     def d(x):
         return x if dlogits == "own" else None
@@ -681,7 +686,7 @@ def test_far_offsets(cuda):
     z = torch.as_strided(buf, (3, V), (ld, 1))
     z.copy_((torch.randn(3, V, generator=gen(5), device="cuda") * 2).bfloat16())
     tokens = tokens_of(3, V, 6)
-    small = z.clone()
+    small = torch.empty(3, V, dtype=BF16, device="cuda").copy_(z)  # rows 16-byte aligned, as z's
     inp = (torch.zeros(3, device="cuda"), torch.ones(3, device="cuda"))
     a = losses.policy_loss(small, tokens, *inp)
     b = losses.policy_loss(z, tokens, *inp, dlogits=z)
