@@ -16,6 +16,9 @@
 // margins are small differences of log-probabilities), and a pass that
 // writes the adjoint.
 #include <cmath>
+#include <cstring>
+#include <mutex>
+#include <set>
 #include <string>
 #include <type_traits>
 
@@ -35,8 +38,8 @@ constexpr int kMaxTeacherK = 1024;
 constexpr int kMaxCluster = 8;
 // Shared memory of a CTA's pieces: three CTAs fit an SM up to kStageBytes,
 // one up to kStageBytesMost.
-constexpr int64_t kStageBytes = 72 * 1024, kStageBytesMost = 200 * 1024;
-constexpr double kLog2e = 1.4426950408889634;
+constexpr int64_t kStageBytes = 68 * 1024, kStageBytesMost = 200 * 1024;
+constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
 struct RowArgs {
   const void* z;
@@ -49,6 +52,7 @@ struct RowArgs {
   double inv_tau;
   float c;       // log2(e) / tau
   int cluster;      // CTAs per row
+  int share;        // 16-byte pieces of a row a CTA has
   int stage_bytes;  // of shared memory for a CTA's pieces
   double scale;  // of the loss and the adjoint
   float* logp;
@@ -66,23 +70,54 @@ struct RowArgs {
   const float* teacher_lse;
 };
 
-// Running maximum and sum of 2^(c (z - max)); a maximum of -inf (no finite
-// element yet) counts as 0, so that 2^(-inf - max) stays 0.  The maximum is
-// subtracted before the factor is applied: c max overflows for a row that is
-// all of the type's lowest value.
+// Powers of two of a row are taken relative to its maximum m as
+// 2^(c z - b) with b = rint(c m), a whole number: one fused multiply-add an
+// element, no rounding of b, and sums with different b differ by exact powers
+// of two.  (c is log2(e) / tau rounded to fp32, for every term of a row alike:
+// a relative change of the temperature by at most 2^-24.)  b is held within
+// +-1e30.  Where c m would pass that, or a row is all of the type's lowest
+// value, two elements are equal or at least 2^60 apart: beyond 1e25 a row is
+// far, and its powers are taken of (z - m) 2^-40, which is exact.
+constexpr float kFar = 1e30f;
+__device__ __forceinline__ float base_of(float m, float c) {
+  return fminf(fmaxf(rintf(c * m), -kFar), kFar);
+}
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > 1e25f && m != -INFINITY; }
+struct Form {
+  float c, b;  // 2^(c z - b)
+};
+__device__ __forceinline__ Form form_of(float m, float c) {
+  if (is_far(m)) return {0x1p-40f, m * 0x1p-40f};
+  return {c, base_of(m, c)};
+}
+// A maximum and the sum of 2^(c z - b) of its form; nothing: {-inf, 0}.
 struct MaxSum {
   float m, s;
 };
-__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
-  const float m = fmaxf(a.m, b.m), k = base_of(m);
-  return {m, a.s * tc::fast_exp2((a.m - k) * c) + b.s * tc::fast_exp2((b.m - k) * c)};
+__device__ __forceinline__ float warp_max_redux(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
+// The warp's maximum and sum; the sum of a far row is not one yet.
 __device__ __forceinline__ MaxSum warp_join(MaxSum v, float c) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    v = join(v, {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o)}, c);
-  return v;
+  const float m = warp_max_redux(v.m);
+  return {m, warp_sum(v.s * tc::fast_exp2(base_of(v.m, c) - base_of(m, c)))};
+}
+// What turns a sum relative to m into one relative to `to` >= m.
+__device__ __forceinline__ float rescale(float m, float to, float c) {
+  if (m == to) return 1.f;
+  if (is_far(m) || is_far(to)) return 0.f;
+  return tc::fast_exp2(base_of(m, c) - base_of(to, c));
+}
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  return {m, a.s * rescale(a.m, m, c) + b.s * rescale(b.m, m, c)};
+}
+// (z - m) / tau, to which log(s) is to be taken from, in double.
+__device__ __forceinline__ double above(float z, float m, float c, double inv_tau) {
+  if (is_far(m)) return ((double)z - (double)m) * inv_tau;
+  return ((double)z * (double)c - (double)base_of(m, c)) * kLn2;
 }
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
@@ -147,59 +182,69 @@ __device__ __forceinline__ void store_unit(bf16* p, const float* v) {
                                             tc::pack_bf16(v[4], v[5]), tc::pack_bf16(v[6], v[7]));
 }
 
-// What the CTAs of a cluster tell one another of their part of the row.
-struct alignas(16) Part {
-  MaxSum rest;    // entries not listed by the teacher (all, elsewhere)
-  MaxSum listed;  // listed entries, each vocabulary entry once
-  float count;    // of the listed entries
-};
-static_assert(sizeof(Part) == 32, "a Part is written to a peer as 16 + 4 bytes");
+// Bits of the filter that finds out whether a list may name an entry twice.
+constexpr int kFilterBits = 32768;
 
-// A cluster of `nctarank` CTAs per row.
+// A cluster of a.cluster CTAs per row.
 template <RowOp OP, typename TI, typename TO>
 __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
   constexpr int EI = 16 / (int)sizeof(TI), EO = 16 / (int)sizeof(TO);
   constexpr int NT = kRowThreads, NW = NT / 32, U = 4;
   extern __shared__ __align__(16) uint8_t dyn[];
-  __shared__ Part s_warp[NW];
-  __shared__ Part s_peer[kMaxCluster];
-  __shared__ double s_red[2][NW];
+  // of every warp of the cluster
+  __shared__ MaxSum s_rest[kMaxCluster * NW];
+  __shared__ float s_again[kMaxCluster * NW];
+  // of every CTA: the listed entries' m, s, count; the sum of q times the logit
+  __shared__ __align__(16) float4 s_listed[kMaxCluster];
+  __shared__ double s_qz[kMaxCluster];
   __shared__ float s_coef[4];
+  __shared__ double s_q[3];
   __shared__ int s_twice;
-  const int C = a.cluster, rank = (int)blockIdx.x % C, tid = threadIdx.x, lane = tid & 31;
-  const int64_t row = blockIdx.x / C;
+  const int C = a.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = (int)tc::cluster_ctarank();
+  uint32_t row32;
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(row32));
+  const int64_t row = row32;
+  const float w = a.weight ? a.weight[row] : 1.f;
+  const int64_t token64 = OP == kDistill ? -1 : a.tokens[row];
+  const float dlogp = OP == kLogpBwd ? a.dlogp[row] : 0.f;
+  const float lse_in = OP == kLogpBwd ? a.lse[row] : 0.f;
+  int32_t my_idx = -1;
+  float my_top = 0.f;
+  if (OP == kDistill && tid < a.K) {
+    my_idx = a.top_index[row * a.K + tid];
+    my_top = a.top_logit[row * a.K + tid];
+  }
+
   const TI* z = (const TI*)a.z + row * a.ld;
   TO* dz = a.dz ? (TO*)a.dz + row * a.ldd : nullptr;
   const int V = (int)a.V;
-  // this CTA's pieces [p0, p1) and elements [e_lo, e_hi)
+  // this CTA's pieces [p0, p0 + np) and elements [e_lo, e_hi)
   const int ph = (int)((uintptr_t)z & 15) / (int)sizeof(TI);
-  const int64_t pieces = ((int64_t)ph + V + EI - 1) / EI;
-  const int p0 = (int)(pieces * rank / C), np = (int)(pieces * (rank + 1) / C) - p0;
-  const int e_org = (int)((int64_t)p0 * EI - ph);  // the row's element at image element 0
-  const int e_lo = max(0, e_org), e_hi = (int)min((int64_t)V, (int64_t)e_org + (int64_t)np * EI);
+  const int pieces = (ph + V + EI - 1) / EI;
+  const int p0 = min(pieces, rank * a.share), np = min(pieces, p0 + a.share) - p0;
+  const int e_org = p0 * EI - ph;  // the row's element at image element 0
+  const int e_lo = max(0, e_org), e_hi = max(e_lo, min(V, e_org + np * EI));
   // units of 16 bytes of dz: whole ones [u0, u1), the rest of the elements ahead and behind
   const int dph = dz ? (int)((uintptr_t)dz & 15) / (int)sizeof(TO) : 0;
-  const int64_t u0 = ((int64_t)dph + e_lo + EO - 1) / EO, u1 = ((int64_t)dph + e_hi) / EO;
-
-  const float w = a.weight ? a.weight[row] : 1.f;
-  const int64_t token = OP == kDistill ? -1 : a.tokens[row];
-  bool skip = w == 0.f || (OP != kDistill && (token < 0 || token >= V));
-  if (OP == kLogpBwd && a.dlogp[row] == 0.f) skip = true;
+  const int u0 = (dph + e_lo + EO - 1) / EO, u1 = (dph + e_hi) / EO;
+  const int token = (int)token64;
 
   // elements of the units that are not whole: f(element)
   auto ragged = [&](auto f) {
     if (u0 >= u1) {
       for (int e = e_lo + tid; e < e_hi; e += NT) f(e);
     } else {
-      const int ahead = (int)(u0 * EO - dph) - e_lo, behind0 = (int)(u1 * EO - dph);
+      const int ahead = u0 * EO - dph - e_lo, behind0 = u1 * EO - dph;
       if (tid < ahead) f(e_lo + tid);
       if (tid >= 32 && tid - 32 < e_hi - behind0) f(behind0 + tid - 32);
     }
   };
-  if (skip) {
+  if (w == 0.f || (OP != kDistill && (token64 < 0 || token64 >= V)) ||
+      (OP == kLogpBwd && dlogp == 0.f)) {
     if (dz) {
       const float zero[EO] = {};
-      for (int64_t u = u0 + tid; u < u1; u += NT) store_unit(dz + (u * EO - dph), zero);
+      for (int u = u0 + tid; u < u1; u += NT) store_unit(dz + (u * EO - dph), zero);
       ragged([&](int e) { st(&dz[e], 0.f); });
     }
     if (tid == 0 && rank == 0) {
@@ -210,206 +255,258 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
     }
     return;
   }
+  // the log-probability's adjoint takes p from lse, but where fp32 does not
+  // hold lse to the digits that p needs
+  const bool stats = OP != kLogpBwd || fabsf(lse_in) > 256.f;
   // every CTA of the cluster has started once this barrier is through: its
   // shared memory may be written to
-  if (OP != kLogpBwd && C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (stats && C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
-  // ---- copy this CTA's pieces
-  const uint32_t img = tc::smem_u32(dyn);
+  // ---- copy this CTA's pieces; thread tid has pieces tid + NT k
   TI* image = (TI*)dyn;
-  const TI* src = z + e_org;
-  const int rounds = (np + U * NT - 1) / (U * NT);
-  for (int r = 0; r < rounds; ++r) {
+  const int mine = tid < np ? (np - tid + NT - 1) / NT : 0;  // how many it has
+  {
+    // the first and the last piece of the row may be in part outside it
+    const int f0 = e_org < 0 ? 1 : 0, f1 = e_org + np * EI > V ? np - 1 : np;
+    auto in_part = [&](int i) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int i = tid + (r * U + j) * NT;
-      if (i >= np) continue;
-      const int e = e_org + i * EI;
-      if (e >= 0 && e <= V - EI) {
-        copy_piece(img + i * 16, src + (int64_t)i * EI);
-      } else {
-        for (int k = 0; k < EI; ++k)
-          image[i * EI + k] = e + k >= 0 && e + k < V ? z[e + k] : (TI)-INFINITY;
+      for (int k = 0; k < EI; ++k) {
+        const int e = e_org + i * EI + k;
+        image[i * EI + k] = e >= 0 && e < V ? z[e] : (TI)-INFINITY;
       }
+    };
+    if (f0 == 1 && tid == 0 && np > 0) in_part(0);
+    if (f1 < np && f1 >= f0 && tid == f1 % NT) in_part(f1);
+    const int i0 = tid < f0 ? tid + NT : tid;
+    const uint32_t dst = tc::smem_u32(dyn) + i0 * 16;
+    const uint4* src = (const uint4*)(z + e_org) + i0;
+    const int n = i0 < f1 ? (f1 - i0 + NT - 1) / NT : 0;
+    int k = 0;
+    for (; k + U <= n; k += U) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) copy_piece(dst + (k + j) * (NT * 16), src + (k + j) * NT);
+      copy_commit();
     }
+    for (; k < n; ++k) copy_piece(dst + k * (NT * 16), src + k * NT);
     copy_commit();
   }
   const float za = OP == kDistill || OP == kLogpBwd ? 0.f : ld(&z[token]);
 
-  // ---- the teacher's entries while the copies run: q, the student's logit
+  // ---- the teacher's entries, while the copies run: q, and which of a
+  // list's entries are a vocabulary entry's first
   int32_t* t_idx = (int32_t*)(dyn + a.stage_bytes);
   float* t_q = (float*)(t_idx + a.K);  // q
-  float* t_z = t_q + a.K;              // the student's logit
+  float* t_z = t_q + a.K;              // the student's logit, of this CTA's entries
   float* t_g = t_z + a.K;              // this CTA's first ones: sum of q of the entry; else -1
-  double q_sum = 0.0, q_logq = 0.0, q_rest = 0.0;
   if (OP == kDistill) {
-    const float* y = a.top_logit + row * a.K;
-    MaxSum t = {-INFINITY, 0.f};
-    for (int k = tid; k < a.K; k += NT) {
-      const int32_t i = a.top_index[row * a.K + k];
-      const bool in = i >= 0 && i < V;
-      const float yk = in ? y[k] : -INFINITY;
-      t_idx[k] = in ? i : -1;
-      t_z[k] = in ? ld(&z[i]) : 0.f;
-      t_q[k] = yk;
-      if (in) t = join(t, {yk, 1.f}, a.c);
-    }
+    uint32_t* filter = (uint32_t*)(t_g + a.K);
+    for (int i = tid; i < kFilterBits / 32; i += NT) filter[i] = 0u;
     if (tid == 0) s_twice = 0;
-    double tl;
-    if (a.teacher_lse) {
-      tl = (double)a.teacher_lse[row];
-    } else {
-      t = warp_join(t, a.c);
-      if (lane == 0) s_warp[tid >> 5].rest = t;
-      __syncthreads();
-      t = s_warp[0].rest;
-      for (int i = 1; i < NW; ++i) t = join(t, s_warp[i].rest, a.c);
-      tl = (double)base_of(t.m) * a.inv_tau + log((double)t.s);
-    }
-    double qs = 0.0, ql = 0.0;
     for (int k = tid; k < a.K; k += NT) {
-      const double lq = (double)t_q[k] * a.inv_tau - tl;
-      const double q = t_idx[k] < 0 || t_q[k] == -INFINITY ? 0.0 : exp(lq);
-      t_q[k] = (float)q;
-      qs += q;
-      if (q > 0.0) ql += q * lq;
-    }
-    qs = warp_sum_d(qs);
-    ql = warp_sum_d(ql);
-    if (lane == 0) {
-      s_red[0][tid >> 5] = qs;
-      s_red[1][tid >> 5] = ql;
-    }
-    // ---- listed entries leave the image: -inf, and each counts once.  A word
-    // of all ones marks an entry; one found marked is named twice (or was that
-    // NaN), and then the entries are compared one by one.
-    copy_wait(0);
-    __syncthreads();
-    for (int i = 0; i < NW; ++i) {
-      q_sum += s_red[0][i];
-      q_logq += s_red[1][i];
-    }
-    q_rest = a.teacher_lse ? fmax(0.0, 1.0 - q_sum) : 0.0;
-    auto here = [&](int k) { return t_idx[k] >= e_lo && t_idx[k] < e_hi; };
-    uint32_t* words = (uint32_t*)dyn;
-    for (int k = tid; k < a.K; k += NT) {
-      t_g[k] = here(k) ? t_q[k] : -1.f;
-      if (!here(k)) continue;
-      const uint32_t at = (uint32_t)(t_idx[k] - e_org) * sizeof(TI);
-      const uint32_t ones = (sizeof(TI) == 4 ? 0xffffffffu : 0xffffu) << (8 * (at & 3));
-      if ((atomicOr(&words[at >> 2], ones) & ones) == ones) s_twice = 1;
+      const int32_t i = k < NT ? my_idx : a.top_index[row * a.K + k];
+      const float y = k < NT ? my_top : a.top_logit[row * a.K + k];
+      const bool in = i >= 0 && i < V;
+      t_idx[k] = in ? i : -1;
+      t_q[k] = in ? y : -INFINITY;
     }
     __syncthreads();
-    for (int k = tid; k < a.K; k += NT) {
-      if (!here(k)) continue;
-      image[t_idx[k] - e_org] = (TI)-INFINITY;
-      if (s_twice) {
-        double g = 0.0;
-        bool first = true;
-        for (int j = 0; j < a.K; ++j)
-          if (t_idx[j] == t_idx[k]) {
-            if (j < k) first = false;
-            g += (double)t_q[j];
-          }
-        t_g[k] = first ? (float)g : -1.f;
+    if (warp == NW - 1) {
+      MaxSum t = {-INFINITY, 0.f};
+      double tl = 0.0;
+      if (a.teacher_lse) {
+        tl = (double)a.teacher_lse[row];
+      } else {
+        for (int k = lane; k < a.K; k += 32) t.m = fmaxf(t.m, t_q[k]);
+        t.m = warp_max_redux(t.m);
+        const Form f = form_of(t.m, a.c);
+        for (int k = lane; k < a.K; k += 32) t.s += tc::fast_exp2(fmaf(t_q[k], f.c, -f.b));
+        tl = log((double)warp_sum(t.s));
+      }
+      double qs = 0.0, ql = 0.0;
+      for (int k = lane; k < a.K; k += 32) {
+        const float y = t_q[k];
+        const double lq = (a.teacher_lse ? (double)y * a.inv_tau : above(y, t.m, a.c, a.inv_tau)) - tl;
+        const float hi = (float)lq;  // q to fp32's last digits: lq rounded, the rest applied
+        const float q = y == -INFINITY ? 0.f : expf(hi) * (1.f + (float)(lq - (double)hi));
+        t_q[k] = q;
+        qs += (double)q;
+        if (q > 0.f) ql += (double)q * lq;
+      }
+      qs = warp_sum_d(qs);
+      ql = warp_sum_d(ql);
+      if (lane == 0) {
+        s_q[0] = qs;
+        s_q[1] = ql;
+        s_q[2] = a.teacher_lse ? fmax(0.0, 1.0 - qs) : 0.0;
       }
     }
+    // two entries on one bit: the list is compared entry by entry
+    for (int k = tid; k < a.K; k += NT)
+      if (t_idx[k] >= 0) {
+        const uint32_t h = (uint32_t)t_idx[k] % kFilterBits, bit = 1u << (h & 31);
+        if (atomicOr(&filter[h >> 5], bit) & bit) s_twice = 1;
+      }
+    // this CTA's entries leave the image
+    copy_wait(0);
+    __syncthreads();
+    for (int k = tid; k < a.K; k += NT) {
+      const int i = t_idx[k];
+      const bool here = i >= e_lo && i < e_hi;
+      float g = here ? t_q[k] : -1.f;
+      if (here && s_twice) {
+        double sum = 0.0;
+        bool first = true;
+        for (int j = 0; j < a.K; ++j)
+          if (t_idx[j] == i) {
+            if (j < k) first = false;
+            sum += (double)t_q[j];
+          }
+        g = first ? (float)sum : -1.f;
+      }
+      t_g[k] = g;
+      t_z[k] = here ? ld(&image[i - e_org]) : 0.f;
+    }
+    __syncthreads();
+    for (int k = tid; k < a.K; k += NT)
+      if (!(t_g[k] < 0.f)) image[t_idx[k] - e_org] = (TI)-INFINITY;
     __syncthreads();
   }
 
   // ---- maximum and sum
-  Part part = {{-INFINITY, 0.f}, {-INFINITY, 0.f}, 0.f};
-  if (OP != kLogpBwd) {
-    float m = -INFINITY;
+  MaxSum rest = {-INFINITY, 0.f}, listed = {-INFINITY, 0.f};
+  float count = 0.f;
+  // v to slot `to` of every CTA of the cluster (lane r: of CTA r)
+  auto tell = [&](auto* to, auto v) {
+    if (C == 1) {
+      if (lane == 0) *to = v;
+    } else if (lane < C) {
+      const uint32_t at = tc::mapa_shared(tc::smem_u32(to), (uint32_t)lane);
+      uint32_t word[sizeof(v) / 4];
+      memcpy(word, &v, sizeof(v));
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(v) / 4; ++i)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + 4 * i), "r"(word[i]) : "memory");
+    }
+  };
+  auto told = [&] {
+    if (C > 1) tc::cluster_sync();
+    else __syncthreads();
+  };
+  if (stats) {
+    const uint4* at = (const uint4*)dyn + tid;
+    float m = -INFINITY, b = base_of(m, a.c);
     float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
     const float2 c2 = make_float2(a.c, a.c);
-    const uint32_t none = minus_inf_word((const TI*)nullptr);
-    for (int r = 0; r < rounds; ++r) {
-      if (OP != kDistill) copy_wait(rounds - 1 - r);
-      float2 x[U][EI / 2];
+    auto take = [&](auto pieces_now, int k) {
+      constexpr int P = decltype(pieces_now)::value;
+      float2 x[P][EI / 2];
       float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = tid + (r * U + j) * NT;
-        const uint4 u = i < np ? ((const uint4*)dyn)[i] : make_uint4(none, none, none, none);
-        unpack(u, x[j], (const TI*)nullptr);
+      for (int j = 0; j < P; ++j) {
+        unpack(at[(k + j) * NT], x[j], (const TI*)nullptr);
 #pragma unroll
-        for (int k = 0; k < EI / 2; ++k) mx = tc::fmax3(mx, x[j][k].x, x[j][k].y);
+        for (int i = 0; i < EI / 2; ++i) mx = tc::fmax3(mx, x[j][i].x, x[j][i].y);
       }
       if (mx > m) {
-        const float k = tc::fast_exp2((m - mx) * a.c);
-        s0 = tc::fmul2(s0, make_float2(k, k));
-        s1 = tc::fmul2(s1, make_float2(k, k));
+        const float nb = base_of(mx, a.c), f = tc::fast_exp2(b - nb);
+        s0 = tc::fmul2(s0, make_float2(f, f));
+        s1 = tc::fmul2(s1, make_float2(f, f));
         m = mx;
+        b = nb;
       }
-      const float2 nb = make_float2(-base_of(m), -base_of(m));
+      const float2 nb = make_float2(-b, -b);
 #pragma unroll
-      for (int j = 0; j < U; ++j)
+      for (int j = 0; j < P; ++j)
 #pragma unroll
-        for (int k = 0; k < EI / 2; ++k) {
-          const float2 t = tc::fmul2(tc::fadd2(x[j][k], nb), c2);
+        for (int i = 0; i < EI / 2; ++i) {
+          const float2 t = tc::ffma2(x[j][i], c2, nb);
           const float2 e = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
-          if (k & 1) s1 = tc::fadd2(s1, e);
+          if (i & 1) s1 = tc::fadd2(s1, e);
           else s0 = tc::fadd2(s0, e);
         }
-    }
-    part.rest = warp_join({m, (s0.x + s0.y) + (s1.x + s1.y)}, a.c);
-    if (OP == kDistill) {
-      MaxSum in = {-INFINITY, 0.f};
-      float n = 0.f;
-      for (int k = tid; k < a.K; k += NT)
-        if (!(t_g[k] < 0.f)) {
-          in = join(in, {t_z[k], t_z[k] == -INFINITY ? 0.f : 1.f}, a.c);
-          n += 1.f;
-        }
-      part.listed = warp_join(in, a.c);
-      part.count = warp_sum(n);
-    }
-    if (lane == 0) s_warp[tid >> 5] = part;
-    __syncthreads();
-    auto add = [&](Part& to, const Part& p) {
-      to.rest = join(to.rest, p.rest, a.c);
-      if (OP == kDistill) {
-        to.listed = join(to.listed, p.listed, a.c);
-        to.count += p.count;
-      }
     };
-    part = s_warp[0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) add(part, s_warp[i]);
-    if (C > 1) {
-      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-      if (tid < C) {
-        const uint32_t to = tc::mapa_shared(tc::smem_u32(&s_peer[rank]), (uint32_t)tid);
-        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to),
-                     "f"(part.rest.m), "f"(part.rest.s), "f"(part.listed.m), "f"(part.listed.s)
-                     : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 16), "f"(part.count) : "memory");
+    int k = 0;
+    for (; k + U <= mine; k += U) {
+      // one copy group has at most U pieces, and group g none behind piece (g + 1) U
+      if (OP != kDistill) copy_wait(max(0, mine / U - 1 - k / U));
+      take(std::integral_constant<int, U>{}, k);
+    }
+    if (OP != kDistill) copy_wait(0);
+    for (; k < mine; ++k) take(std::integral_constant<int, 1>{}, k);
+    rest = warp_join({m, (s0.x + s0.y) + (s1.x + s1.y)}, a.c);
+    double qz = 0.0;
+    if (OP == kDistill && warp == NW - 1) {
+      for (int k = lane; k < a.K; k += 32) {
+        const int i = t_idx[k];
+        if (i >= e_lo && i < e_hi && t_q[k] != 0.f) qz += (double)t_q[k] * (double)t_z[k];
+        if (t_g[k] < 0.f) continue;
+        listed.m = fmaxf(listed.m, t_z[k]);
+        count += 1.f;
       }
-      tc::cluster_sync();
-      part = s_peer[0];
-      for (int i = 1; i < C; ++i) add(part, s_peer[i]);
+      qz = warp_sum_d(qz);
+      listed.m = warp_max_redux(listed.m);
+      const Form f = form_of(listed.m, a.c);
+      for (int k = lane; k < a.K; k += 32)
+        if (!(t_g[k] < 0.f)) listed.s += tc::fast_exp2(fmaf(t_z[k], f.c, -f.b));
+      listed.s = warp_sum(listed.s);
+      count = warp_sum(count);
+    }
+    // every warp's to every CTA of the cluster, joined there in a fixed order
+    if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    tell(&s_rest[rank * NW + warp], rest);
+    if (OP == kDistill && warp == NW - 1) {
+      tell(&s_listed[rank], make_float4(listed.m, listed.s, count, 0.f));
+      tell(&s_qz[rank], qz);
+    }
+    told();
+    rest = {-INFINITY, 0.f};
+    if (lane < C * NW) rest = s_rest[lane];
+    if (C * NW > 32 && lane + 32 < C * NW) rest = join(rest, s_rest[lane + 32], a.c);
+    rest = warp_join(rest, a.c);
+    if (is_far(rest.m)) {
+      const Form f = form_of(rest.m, a.c);
+      float s = 0.f;
+      for (k = 0; k < mine; ++k) {
+        float2 x[EI / 2];
+        unpack(at[k * NT], x, (const TI*)nullptr);
+#pragma unroll
+        for (int i = 0; i < EI / 2; ++i)
+          s += tc::fast_exp2(fmaf(x[i].x, f.c, -f.b)) + tc::fast_exp2(fmaf(x[i].y, f.c, -f.b));
+      }
+      tell(&s_again[rank * NW + warp], warp_sum(s));
+      told();
+      s = lane < C * NW ? s_again[lane] : 0.f;
+      if (C * NW > 32 && lane + 32 < C * NW) s += s_again[lane + 32];
+      rest.s = warp_sum(s);
+    }
+    if (OP == kDistill) {
+      listed = {-INFINITY, 0.f};
+      count = 0.f;
+      for (int i = 0; i < C; ++i) {
+        listed = join(listed, {s_listed[i].x, s_listed[i].y}, a.c);
+        count += s_listed[i].z;
+      }
     }
   }
-  const MaxSum r = part.rest;
 
-  // ---- the row's scalars: dz = c_out 2^((f z - b) c) + corrections
-  float c_in = 0.f, b_in = 0.f, c_out = 0.f, hot = 0.f, b = base_of(r.m), f = 1.f, c = a.c;
+  // ---- the row's scalars: dz = c_out 2^(c z - b) + corrections, in the form
+  // of the maximum outside the list
+  Form f = form_of(rest.m, a.c), f_in = f;
+  float c_in = 0.f, c_out = 0.f, hot = 0.f;
   if (OP == kLogpBwd) {
-    hot = (float)((double)a.dlogp[row] * a.inv_tau);
-    c_out = -hot;
-    f = (float)a.inv_tau;
-    b = a.lse[row];
-    c = (float)kLog2e;
+    const double g = (double)dlogp * a.inv_tau;
+    hot = (float)g;
+    if (stats) {
+      c_out = (float)(-g / (double)rest.s);
+    } else {
+      // 2^(c z - log2(e) lse): the whole part stays in the exponent
+      const double l2 = (double)lse_in * kLog2e;
+      f.b = (float)rint(l2);
+      c_out = -hot * tc::fast_exp2((float)((double)f.b - l2));
+    }
   } else if (OP != kDistill) {
     if (tid == 0) {
-      const double ls = log((double)r.s);
-      const double logp = ((double)za - (double)b) * a.inv_tau - ls;
-      if (rank == 0) {
-        if (a.logp) a.logp[row] = (float)logp;
-        if (OP == kLogp && a.logp_lo) a.logp_lo[row] = (float)(logp - (double)(float)logp);
-        if (OP == kLogp && a.lse) a.lse[row] = (float)((double)b * a.inv_tau + ls);
-      }
+      const double ls = log((double)rest.s), logp = above(za, rest.m, a.c, a.inv_tau) - ls;
       if (OP == kPolicy) {
         const double A = a.advantage[row], ratio = exp(logp - (double)a.old_logp[row]);
         const double lo = 1.0 - a.clip_low, hi = 1.0 + a.clip_high;
@@ -424,7 +521,12 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
         if (rank == 0) a.row_loss[row] = (float)((double)w * l);
         const double g = a.scale * (double)w * d * a.inv_tau;
         s_coef[0] = (float)g;
-        s_coef[1] = (float)(-g / (double)r.s);
+        s_coef[1] = (float)(-g / (double)rest.s);
+      }
+      if (rank == 0) {
+        if (a.logp) a.logp[row] = (float)logp;
+        if (OP == kLogp && a.logp_lo) a.logp_lo[row] = (float)(logp - (double)(float)logp);
+        if (OP == kLogp && a.lse) a.lse[row] = (float)(ls - above(0.f, rest.m, a.c, a.inv_tau));
       }
     }
     if (OP == kLogp || !dz) return;
@@ -432,35 +534,44 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
     hot = s_coef[0];
     c_out = s_coef[1];
   } else {
-    const MaxSum all = join(r, part.listed, a.c);
+    const MaxSum all = join(rest, listed, a.c);
+    f_in = form_of(all.m, a.c);
     // without an entry outside the list there is no class for the rest
-    if (part.count == (float)V) q_rest = 0.0;
-    const double ls = log((double)all.s), mx = (double)base_of(all.m) * a.inv_tau;
-    double cross = 0.0;
-    for (int k = tid; k < a.K; k += NT)
-      if (t_q[k] != 0.f) cross += (double)t_q[k] * ((double)t_z[k] * a.inv_tau - mx - ls);
-    if (rank == 0) {
-      cross = block_sum_d(cross, s_red[0]);
-      if (tid == 0) {
-        double l = q_logq - cross;
-        if (q_rest > 0.0)
-          l += q_rest *
-               (log(q_rest) - ((double)b * a.inv_tau + log((double)r.s) - mx - ls));
+    const double q_sum = s_q[0], q_rest = count == (float)V ? 0.0 : s_q[2];
+    if (tid == 0) {
+      const double g = a.scale * (double)w / a.inv_tau, Q = q_sum + q_rest;
+      const double in = Q / (double)all.s;
+      s_coef[0] = (float)g;
+      s_coef[1] = (float)(g * in);
+      // outside the list relative to the largest logit there: the student's
+      // mass outside may be too small to be held relative to the row's
+      // largest (none at all: an infinite loss, and entries of probability 0)
+      s_coef[2] = rest.s == 0.f ? (all.s == 0.f ? NAN : 0.f)
+                                : (float)(g * (in * (double)rescale(rest.m, all.m, a.c) -
+                                               (q_rest > 0.0 ? q_rest / (double)rest.s : 0.0)));
+    }
+    // the loss, by a warp that writes its part of the adjoint later
+    if (warp == NW - 1 && rank == 0) {
+      const double ls = log((double)(lane == 0 ? all.s : lane == 1 ? rest.s : (float)q_rest));
+      const double ls_all = __shfl_sync(0xffffffffu, ls, 0), ls_rest = __shfl_sync(0xffffffffu, ls, 1);
+      if (lane == 2) {
+        double qz_all = 0.0;
+        for (int i = 0; i < C; ++i) qz_all += s_qz[i];
+        // sum of q (z / tau - lse), as above() has it of one z
+        const double x = is_far(all.m) ? (qz_all - q_sum * (double)all.m) * a.inv_tau
+                                       : (qz_all * (double)a.c - q_sum * (double)f_in.b) * kLn2;
+        double l = s_q[1] - (x - q_sum * ls_all);
+        if (q_rest > 0.0)  // -log of the student's share outside the list
+          l += q_rest * (ls + (ls_all - above(0.f, all.m, a.c, a.inv_tau)) -
+                         (ls_rest - above(0.f, rest.m, a.c, a.inv_tau)));
         a.row_loss[row] = (float)((double)w * l / (a.inv_tau * a.inv_tau));
       }
     }
     if (!dz) return;
-    const double g = a.scale * (double)w / a.inv_tau;
-    const double Q = q_sum + q_rest;
-    c_in = (float)(g * Q / (double)all.s);
-    b_in = base_of(all.m);
-    // outside the list relative to the largest logit there: the student's
-    // mass outside may be too small to be held relative to the row's largest
-    // (none at all: an infinite loss, and entries of probability 0)
-    c_out = r.s == 0.f ? 0.f
-                       : (float)(g * (Q * (double)tc::fast_exp2((b - b_in) * a.c) / (double)all.s -
-                                      (q_rest > 0.0 ? q_rest / (double)r.s : 0.0)));
-    hot = (float)g;
+    __syncthreads();
+    hot = s_coef[0];
+    c_in = s_coef[1];
+    c_out = s_coef[2];
   }
 
   // ---- the adjoint, in 16-byte units of dz; an image whose pieces do not
@@ -469,50 +580,54 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
     copy_wait(0);
     __syncthreads();
   }
-  const float2 f2 = make_float2(f, f), nb = make_float2(-b, -b), c2 = make_float2(c, c);
-  auto value = [&](float x) { return c_out * tc::fast_exp2(fmaf(x, f, -b) * c); };
-  const bool aligned = ((int)(u0 * EO - dph) - e_org) % EI == 0;
-  auto unit = [&](int64_t u, auto lined_up) {
-    const int e0 = (int)(u * EO - dph), at = e0 - e_org;
-    float2 x[EO / 2];
-    float v[EO];
-    if constexpr (decltype(lined_up)::value) {
+  const float2 c2 = make_float2(f.c, f.c), nb = make_float2(-f.b, -f.b);
+  const float2 g2 = make_float2(c_out, c_out);
+  const int first = u0 + tid, at0 = first * EO - dph - e_org;
+  TO* out = dz + (first * EO - dph);
+  int to_token = token - (first * EO - dph);
+  auto units = [&](auto lined_up) {
+    const TI* in = image + at0;
+#pragma unroll 2
+    for (int u = first; u < u1; u += NT) {
+      float2 x[EO / 2];
+      if constexpr (decltype(lined_up)::value) {
 #pragma unroll
-      for (int q = 0; q < EO / EI; ++q)
-        unpack(((const uint4*)dyn)[at / EI + q], &x[q * (EI / 2)], (const TI*)nullptr);
-    } else {
+        for (int k = 0; k < EO / EI; ++k)
+          unpack(((const uint4*)in)[k], &x[k * (EI / 2)], (const TI*)nullptr);
+      } else {
 #pragma unroll
-      for (int k = 0; k < EO / 2; ++k) x[k] = make_float2(ld(&image[at + 2 * k]), ld(&image[at + 2 * k + 1]));
-    }
+        for (int k = 0; k < EO / 2; ++k) x[k] = make_float2(ld(&in[2 * k]), ld(&in[2 * k + 1]));
+      }
+      float v[EO];
 #pragma unroll
-    for (int k = 0; k < EO / 2; ++k) {
-      const float2 t = tc::fmul2(OP == kLogpBwd ? tc::ffma2(x[k], f2, nb) : tc::fadd2(x[k], nb), c2);
-      v[2 * k] = c_out * tc::fast_exp2(t.x);
-      v[2 * k + 1] = c_out * tc::fast_exp2(t.y);
-    }
-    if (OP != kDistill) {
-      const int64_t d = token - e0;
-      if (d >= 0 && d < EO) {
+      for (int k = 0; k < EO / 2; ++k) {
+        const float2 t = tc::ffma2(x[k], c2, nb);
+        const float2 d = tc::fmul2(make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y)), g2);
+        v[2 * k] = d.x;
+        v[2 * k + 1] = d.y;
+      }
+      if (OP != kDistill && (unsigned)to_token < (unsigned)EO) {
 #pragma unroll
         for (int k = 0; k < EO; ++k)
-          if (d == k) v[k] += hot;
+          if (to_token == k) v[k] += hot;
       }
+      store_unit(out, v);
+      in += NT * EO;
+      out += NT * EO;
+      to_token -= NT * EO;
     }
-    store_unit(dz + e0, v);
   };
-  if (aligned) {
-#pragma unroll 2
-    for (int64_t u = u0 + tid; u < u1; u += NT) unit(u, std::true_type{});
-  } else {
-#pragma unroll 2
-    for (int64_t u = u0 + tid; u < u1; u += NT) unit(u, std::false_type{});
-  }
-  ragged([&](int e) { st(&dz[e], value(ld(&image[e - e_org])) + (e == token ? hot : 0.f)); });
+  if ((u0 * EO - dph - e_org) % EI == 0) units(std::true_type{});
+  else units(std::false_type{});
+  ragged([&](int e) {
+    const float d = c_out * tc::fast_exp2(fmaf(ld(&image[e - e_org]), f.c, -f.b));
+    st(&dz[e], OP != kDistill && e == token ? d + hot : d);
+  });
   if (OP == kDistill) {
     __syncthreads();
     for (int k = tid; k < a.K; k += NT)
       if (!(t_g[k] < 0.f))
-        st(&dz[t_idx[k]], c_in * tc::fast_exp2((t_z[k] - b_in) * c) - hot * t_g[k]);
+        st(&dz[t_idx[k]], c_in * tc::fast_exp2(fmaf(t_z[k], f_in.c, -f_in.b)) - hot * t_g[k]);
   }
 }
 
@@ -586,37 +701,59 @@ __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_co
 }
 
 // ------------------------------------------------------------------- host
+// Let a kernel use the shared memory it may need, once per device.
+void allow_shared_memory(const void* kern) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void*>> done;
+  int dev = 0;
+  DOP_CHECK_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done.count({dev, kern})) {
+    DOP_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)(kStageBytesMost + 16 * kMaxTeacherK + kFilterBits / 8)));
+    done.insert({dev, kern});
+  }
+}
+
+// How the rows are laid out over CTAs: as few of them per row as hold its
+// 16-byte pieces in kStageBytes each, and at most kMaxCluster.
+struct Split {
+  int cluster, share;  // CTAs per row; pieces per CTA
+};
+Split split_of(int64_t rows, int64_t vocab, int prec) {
+  // the pieces that a row touches wherever it starts
+  const int64_t size = prec == DOP_BF16 ? 2 : 4, pieces = ceil_div(vocab * size + 16 - size, 16);
+  const int64_t C = std::min<int64_t>(ceil_div(16 * pieces, kStageBytes), kMaxCluster);
+  const int64_t share = ceil_div(pieces, C);
+  if (16 * share > kStageBytesMost)
+    throw Error(DOP_E_UNSUPPORTED, "vocab (" + std::to_string(vocab) + ") is above " +
+                                       std::to_string((C * kStageBytesMost - 16) / size + 1));
+  if (rows * C > INT32_MAX) throw Error(DOP_E_UNSUPPORTED, "too many rows for this vocab");
+  return {(int)C, (int)share};
+}
+
 template <RowOp OP>
 void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t s) {
   if (rows == 0) return;
-  const int64_t bytes = a.V * (prec == DOP_BF16 ? 2 : 4) + 16;
-  int64_t C = ceil_div(bytes, kStageBytes);
-  if (C > kMaxCluster) {
-    C = kMaxCluster;
-    if (ceil_div(bytes, C) > kStageBytesMost - 16)
-      throw Error(DOP_E_UNSUPPORTED, "vocab (" + std::to_string(a.V) + ") is above " +
-                                         std::to_string(kMaxCluster * (kStageBytesMost - 32) /
-                                                        (prec == DOP_BF16 ? 2 : 4)));
-  }
-  if (rows * C > INT32_MAX) throw Error(DOP_E_UNSUPPORTED, "too many rows for this vocab");
-  a.cluster = (int)C;
-  a.stage_bytes = (int)round_up(ceil_div(bytes, C) + 16, 16);
-  const size_t smem = (size_t)a.stage_bytes + (OP == kDistill ? 16 * (size_t)a.K : 0);
+  const Split sp = split_of(rows, a.V, prec);
+  a.cluster = sp.cluster;
+  a.share = sp.share;
+  a.stage_bytes = 16 * sp.share;
+  const size_t smem = (size_t)a.stage_bytes + (OP == kDistill ? 16 * (size_t)a.K + kFilterBits / 8 : 0);
   auto go = [&](auto ti, auto to) {
     auto kern = k_vocab_row<OP, decltype(ti), decltype(to)>;
-    DOP_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(kStageBytesMost + 16 * kMaxTeacherK)));
+    allow_shared_memory((const void*)kern);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * C));
+    cfg.gridDim = dim3((unsigned)(rows * a.cluster));
     cfg.blockDim = dim3(kRowThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)C;
+    at[0].val.clusterDim.x = (unsigned)a.cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = C > 1 ? 1 : 0;
+    cfg.numAttrs = 1;
     DOP_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   };
   if (prec == DOP_BF16) go(bf16{}, bf16{});
@@ -631,10 +768,11 @@ void check_rows(int64_t rows, int64_t vocab, int prec, const void* z, int64_t ld
   DOP_REQUIRE(rows >= 0 && rows <= INT32_MAX, "rows must lie in [0, 2^31)");
   DOP_REQUIRE(vocab >= 1 && vocab <= INT32_MAX, "vocab must lie in [1, 2^31)");
   DOP_REQUIRE(prec == DOP_F32 || prec == DOP_BF16, "unknown precision");
+  split_of(rows, vocab, prec);
   DOP_REQUIRE(ld >= vocab, "the logits' row stride is smaller than vocab");
   DOP_REQUIRE(z || rows == 0, "null logits");
   DOP_REQUIRE((uintptr_t)z % elem_bytes(prec) == 0, "misaligned logits");
-  DOP_REQUIRE(std::isfinite(tau) && tau > 0.0, "temperature must be finite and positive");
+  DOP_REQUIRE(tau >= 0x1p-16 && tau <= 0x1p16, "temperature must lie in [2^-16, 2^16]");
 }
 // dlogits: bf16 or the logits' type; either exactly the logits' memory (same
 // type and stride) or apart from it.

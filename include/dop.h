@@ -315,8 +315,8 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  * the loss and its adjoint dlogits, which dop_model_backward takes.  They have
  * no counterpart in the crate.  Conventions of all of them:
  *
- *   - x = z / temperature, lse = log sum exp x, p = exp(x - lse).  Row r starts
- *     at logits + r * ld elements (ld >= vocab).  `precision` is the logits'
+ *   - x = z / temperature (between 2^-16 and 2^16), lse = log sum exp x,
+ *     p = exp(x - lse).  Row r starts at logits + r * ld elements (ld >= vocab).  `precision` is the logits'
  *     type; dlogits has `grad_precision`: DOP_BF16, or DOP_F32 for fp32 logits.
  *     dlogits may be the logits' own memory when type and stride are the same
  *     (ldd == ld); any other overlap is refused.  dlogits is ASSIGNED, all of
