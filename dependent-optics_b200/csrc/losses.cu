@@ -36,9 +36,9 @@ enum RowOp : int { kLogp = 0, kLogpBwd = 1, kPolicy = 2, kDistill = 3 };
 constexpr int kRowThreads = 256;
 constexpr int kMaxTeacherK = 1024;
 constexpr int kMaxCluster = 8;
-// Shared memory of a CTA's pieces: three CTAs fit an SM up to kStageBytes,
-// one up to kStageBytesMost.
-constexpr int64_t kStageBytes = 68 * 1024, kStageBytesMost = 200 * 1024;
+// Shared memory: of a CTA when three are to fit an SM (of its 228 KB, less the
+// static share and what the system takes of each), and of a CTA's pieces at most.
+constexpr int64_t kCtaBytes = 228 * 1024 / 3 - 2560, kStageBytesMost = 200 * 1024;
 constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
 struct RowArgs {
@@ -174,21 +174,39 @@ __device__ __forceinline__ void unpack(uint4 u, float2* x, const bf16*) {
 }
 __device__ __forceinline__ uint32_t minus_inf_word(const float*) { return 0xff800000u; }
 __device__ __forceinline__ uint32_t minus_inf_word(const bf16*) { return 0xff80ff80u; }
-__device__ __forceinline__ void store_unit(float* p, const float* v) {
+// N consecutive elements (N sizeof(T) is 8 or 16, and aligned to that).
+__device__ __forceinline__ void store_n(float* p, const float (&v)[4]) {
   *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
-__device__ __forceinline__ void store_unit(bf16* p, const float* v) {
+__device__ __forceinline__ void store_n(bf16* p, const float (&v)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(tc::pack_bf16(v[0], v[1]), tc::pack_bf16(v[2], v[3]));
+}
+__device__ __forceinline__ void store_n(bf16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(tc::pack_bf16(v[0], v[1]), tc::pack_bf16(v[2], v[3]),
                                             tc::pack_bf16(v[4], v[5]), tc::pack_bf16(v[6], v[7]));
 }
 
 // Bits of the filter that finds out whether a list may name an entry twice.
 constexpr int kFilterBits = 32768;
+// A list's arrays start at 16-byte borders.
+__host__ __device__ constexpr int list_stride(int K) { return (K + 3) & ~3; }
 
-// A cluster of a.cluster CTAs per row.
+// ln(s), to about 2^-24 of it or of 1: the exponent apart (0, subnormal, inf
+// and NaN as log has them).
+__device__ __forceinline__ double ln(float s) {
+  if (!(s > 0x1p-126f && s < INFINITY)) return (double)logf(s);
+  const int e = (__float_as_int(s) - 0x3f400000) >> 23;  // s = 2^e f, f in [0.75, 1.5)
+  return (double)e * kLn2 + (double)logf(__int_as_float(__float_as_int(s) - (e << 23)));
+}
+
+// A cluster of a.cluster CTAs per row: 256 threads own the pieces, and
+// distillation has a warp more for the teacher's list.
+template <RowOp OP>
+constexpr int kThreadsOf = kRowThreads + (OP == kDistill ? 32 : 0);
+
 template <RowOp OP, typename TI, typename TO>
-__global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
-  constexpr int EI = 16 / (int)sizeof(TI), EO = 16 / (int)sizeof(TO);
+__global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a) {
+  constexpr int EI = 16 / (int)sizeof(TI);
   constexpr int NT = kRowThreads, NW = NT / 32, U = 4;
   extern __shared__ __align__(16) uint8_t dyn[];
   // of every warp of the cluster
@@ -197,10 +215,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
   // of every CTA: the listed entries' m, s, count; the sum of q times the logit
   __shared__ __align__(16) float4 s_listed[kMaxCluster];
   __shared__ double s_qz[kMaxCluster];
-  __shared__ float s_coef[4];
   __shared__ double s_q[3];
   __shared__ int s_twice;
   const int C = a.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool owner = OP != kDistill || tid < NT;  // of pieces
   const int rank = (int)tc::cluster_ctarank();
   uint32_t row32;
   asm("mov.u32 %0, %%clusterid.x;" : "=r"(row32));
@@ -209,43 +227,33 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
   const int64_t token64 = OP == kDistill ? -1 : a.tokens[row];
   const float dlogp = OP == kLogpBwd ? a.dlogp[row] : 0.f;
   const float lse_in = OP == kLogpBwd ? a.lse[row] : 0.f;
-  int32_t my_idx = -1;
-  float my_top = 0.f;
-  if (OP == kDistill && tid < a.K) {
-    my_idx = a.top_index[row * a.K + tid];
-    my_top = a.top_logit[row * a.K + tid];
-  }
+  const float adv = OP == kPolicy ? a.advantage[row] : 0.f;
+  const float old_logp = OP == kPolicy ? a.old_logp[row] : 0.f;
+  const float ref_logp = OP == kPolicy && a.ref_logp ? a.ref_logp[row] : 0.f;
 
   const TI* z = (const TI*)a.z + row * a.ld;
   TO* dz = a.dz ? (TO*)a.dz + row * a.ldd : nullptr;
-  const int V = (int)a.V;
+  const int V = (int)a.V, token = (int)token64;
   // this CTA's pieces [p0, p0 + np) and elements [e_lo, e_hi)
   const int ph = (int)((uintptr_t)z & 15) / (int)sizeof(TI);
   const int pieces = (ph + V + EI - 1) / EI;
   const int p0 = min(pieces, rank * a.share), np = min(pieces, p0 + a.share) - p0;
   const int e_org = p0 * EI - ph;  // the row's element at image element 0
   const int e_lo = max(0, e_org), e_hi = max(e_lo, min(V, e_org + np * EI));
-  // units of 16 bytes of dz: whole ones [u0, u1), the rest of the elements ahead and behind
-  const int dph = dz ? (int)((uintptr_t)dz & 15) / (int)sizeof(TO) : 0;
-  const int u0 = (dph + e_lo + EO - 1) / EO, u1 = (dph + e_hi) / EO;
-  const int token = (int)token64;
+  // pieces that lie in the row altogether: [f0, f1)
+  const int f0 = e_org < 0 ? 1 : 0, f1 = e_org + np * EI > V ? np - 1 : np;
 
-  // elements of the units that are not whole: f(element)
-  auto ragged = [&](auto f) {
-    if (u0 >= u1) {
-      for (int e = e_lo + tid; e < e_hi; e += NT) f(e);
-    } else {
-      const int ahead = u0 * EO - dph - e_lo, behind0 = u1 * EO - dph;
-      if (tid < ahead) f(e_lo + tid);
-      if (tid >= 32 && tid - 32 < e_hi - behind0) f(behind0 + tid - 32);
-    }
-  };
   if (w == 0.f || (OP != kDistill && (token64 < 0 || token64 >= V)) ||
       (OP == kLogpBwd && dlogp == 0.f)) {
     if (dz) {
-      const float zero[EO] = {};
-      for (int u = u0 + tid; u < u1; u += NT) store_unit(dz + (u * EO - dph), zero);
-      ragged([&](int e) { st(&dz[e], 0.f); });
+      constexpr int EO = 16 / (int)sizeof(TO);
+      const int dph = (int)((uintptr_t)dz & 15) / (int)sizeof(TO);
+      const int u0 = (dph + e_lo + EO - 1) / EO, u1 = (dph + e_hi) / EO;  // 16-byte units
+      const int ahead = u0 < u1 ? u0 * EO - dph : e_hi, behind = u0 < u1 ? u1 * EO - dph : e_hi;
+      for (int u = u0 + tid; u < u1; u += kThreadsOf<OP>)
+        *reinterpret_cast<uint4*>(dz + (u * EO - dph)) = make_uint4(0u, 0u, 0u, 0u);
+      if (e_lo + tid < ahead) st(&dz[e_lo + tid], 0.f);
+      if (behind + tid < e_hi) st(&dz[behind + tid], 0.f);
     }
     if (tid == 0 && rank == 0) {
       if (OP != kLogpBwd && OP != kDistill && a.logp) a.logp[row] = 0.f;
@@ -262,12 +270,13 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
   // shared memory may be written to
   if (stats && C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
-  // ---- copy this CTA's pieces; thread tid has pieces tid + NT k
+  // ---- copy this CTA's pieces; a thread owns pieces tid + NT k, and the
+  // first `mine` of them are the row's
   TI* image = (TI*)dyn;
-  const int mine = tid < np ? (np - tid + NT - 1) / NT : 0;  // how many it has
-  {
+  uint4* at = (uint4*)dyn + tid;  // piece k: at[k NT]
+  const int mine = owner && tid < np ? (np - tid + NT - 1) / NT : 0;
+  if (owner) {
     // the first and the last piece of the row may be in part outside it
-    const int f0 = e_org < 0 ? 1 : 0, f1 = e_org + np * EI > V ? np - 1 : np;
     auto in_part = [&](int i) {
 #pragma unroll
       for (int k = 0; k < EI; ++k) {
@@ -292,35 +301,44 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
   }
   const float za = OP == kDistill || OP == kLogpBwd ? 0.f : ld(&z[token]);
 
-  // ---- the teacher's entries, while the copies run: q, and which of a
-  // list's entries are a vocabulary entry's first
+  // ---- the teacher's list, by the warp that owns no pieces while the others
+  // wait for theirs: q, and which entries are a vocabulary entry's first
+  const int K4 = OP == kDistill ? list_stride(a.K) : 0;
   int32_t* t_idx = (int32_t*)(dyn + a.stage_bytes);
-  float* t_q = (float*)(t_idx + a.K);  // q
-  float* t_z = t_q + a.K;              // the student's logit, of this CTA's entries
-  float* t_g = t_z + a.K;              // this CTA's first ones: sum of q of the entry; else -1
+  float* t_q = (float*)t_idx + K4;  // q
+  float* t_z = t_q + K4;            // the student's logit, of this CTA's entries
+  float* t_g = t_z + K4;            // this CTA's first ones: sum of q of the entry; else -1
   if (OP == kDistill) {
-    uint32_t* filter = (uint32_t*)(t_g + a.K);
-    for (int i = tid; i < kFilterBits / 32; i += NT) filter[i] = 0u;
-    if (tid == 0) s_twice = 0;
-    for (int k = tid; k < a.K; k += NT) {
-      const int32_t i = k < NT ? my_idx : a.top_index[row * a.K + k];
-      const float y = k < NT ? my_top : a.top_logit[row * a.K + k];
-      const bool in = i >= 0 && i < V;
-      t_idx[k] = in ? i : -1;
-      t_q[k] = in ? y : -INFINITY;
-    }
-    __syncthreads();
-    if (warp == NW - 1) {
+    if (!owner) {
+      uint32_t* filter = (uint32_t*)(t_g + K4);
+      const int32_t* index = a.top_index + row * a.K;
+      const float* top = a.top_logit + row * a.K;
+      const double tl_given = a.teacher_lse ? (double)a.teacher_lse[row] : 0.0;
+      for (int i = lane; i < kFilterBits / 128; i += 32) ((uint4*)filter)[i] = make_uint4(0u, 0u, 0u, 0u);
       MaxSum t = {-INFINITY, 0.f};
-      double tl = 0.0;
-      if (a.teacher_lse) {
-        tl = (double)a.teacher_lse[row];
-      } else {
-        for (int k = lane; k < a.K; k += 32) t.m = fmaxf(t.m, t_q[k]);
+      for (int k = lane; k < a.K; k += 32) {
+        const int32_t i = index[k];
+        const float y = top[k];
+        const bool in = i >= 0 && i < V;
+        t_idx[k] = in ? i : -1;
+        t_q[k] = in ? y : -INFINITY;
+        if (in) t.m = fmaxf(t.m, y);
+      }
+      __syncwarp();
+      // two entries on one bit: the list is compared entry by entry
+      bool twice = false;
+      for (int k = lane; k < a.K; k += 32)
+        if (t_idx[k] >= 0) {
+          const uint32_t h = (uint32_t)t_idx[k] % kFilterBits, bit = 1u << (h & 31);
+          if (atomicOr(&filter[h >> 5], bit) & bit) twice = true;
+        }
+      twice = __any_sync(0xffffffffu, twice);
+      double tl = tl_given;
+      if (!a.teacher_lse) {
         t.m = warp_max_redux(t.m);
         const Form f = form_of(t.m, a.c);
         for (int k = lane; k < a.K; k += 32) t.s += tc::fast_exp2(fmaf(t_q[k], f.c, -f.b));
-        tl = log((double)warp_sum(t.s));
+        tl = ln(warp_sum(t.s));
       }
       double qs = 0.0, ql = 0.0;
       for (int k = lane; k < a.K; k += 32) {
@@ -328,48 +346,49 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
         const double lq = (a.teacher_lse ? (double)y * a.inv_tau : above(y, t.m, a.c, a.inv_tau)) - tl;
         const float hi = (float)lq;  // q to fp32's last digits: lq rounded, the rest applied
         const float q = y == -INFINITY ? 0.f : expf(hi) * (1.f + (float)(lq - (double)hi));
+        const bool here = t_idx[k] >= e_lo && t_idx[k] < e_hi;
         t_q[k] = q;
+        t_g[k] = here ? q : -1.f;
         qs += (double)q;
         if (q > 0.f) ql += (double)q * lq;
       }
       qs = warp_sum_d(qs);
       ql = warp_sum_d(ql);
+      __syncwarp();
+      if (twice)
+        for (int k = lane; k < a.K; k += 32) {
+          const int i = t_idx[k];
+          if (t_g[k] < 0.f) continue;
+          double sum = 0.0;
+          bool first = true;
+          for (int j = 0; j < a.K; ++j)
+            if (t_idx[j] == i) {
+              if (j < k) first = false;
+              sum += (double)t_q[j];
+            }
+          t_g[k] = first ? (float)sum : -1.f;
+        }
       if (lane == 0) {
         s_q[0] = qs;
         s_q[1] = ql;
         s_q[2] = a.teacher_lse ? fmax(0.0, 1.0 - qs) : 0.0;
+        s_twice = twice;
       }
     }
-    // two entries on one bit: the list is compared entry by entry
-    for (int k = tid; k < a.K; k += NT)
-      if (t_idx[k] >= 0) {
-        const uint32_t h = (uint32_t)t_idx[k] % kFilterBits, bit = 1u << (h & 31);
-        if (atomicOr(&filter[h >> 5], bit) & bit) s_twice = 1;
-      }
     // this CTA's entries leave the image
     copy_wait(0);
     __syncthreads();
-    for (int k = tid; k < a.K; k += NT) {
-      const int i = t_idx[k];
-      const bool here = i >= e_lo && i < e_hi;
-      float g = here ? t_q[k] : -1.f;
-      if (here && s_twice) {
-        double sum = 0.0;
-        bool first = true;
-        for (int j = 0; j < a.K; ++j)
-          if (t_idx[j] == i) {
-            if (j < k) first = false;
-            sum += (double)t_q[j];
-          }
-        g = first ? (float)sum : -1.f;
-      }
-      t_g[k] = g;
-      t_z[k] = here ? ld(&image[i - e_org]) : 0.f;
+    for (int k = tid; k < a.K; k += kThreadsOf<OP>) {
+      const bool here = t_idx[k] >= e_lo && t_idx[k] < e_hi;
+      t_z[k] = here ? ld(&image[t_idx[k] - e_org]) : 0.f;
+      if (!s_twice && here) image[t_idx[k] - e_org] = (TI)-INFINITY;
     }
     __syncthreads();
-    for (int k = tid; k < a.K; k += NT)
-      if (!(t_g[k] < 0.f)) image[t_idx[k] - e_org] = (TI)-INFINITY;
-    __syncthreads();
+    if (s_twice) {
+      for (int k = tid; k < a.K; k += kThreadsOf<OP>)
+        if (!(t_g[k] < 0.f)) image[t_idx[k] - e_org] = (TI)-INFINITY;
+      __syncthreads();
+    }
   }
 
   // ---- maximum and sum
@@ -380,12 +399,12 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
     if (C == 1) {
       if (lane == 0) *to = v;
     } else if (lane < C) {
-      const uint32_t at = tc::mapa_shared(tc::smem_u32(to), (uint32_t)lane);
+      const uint32_t there = tc::mapa_shared(tc::smem_u32(to), (uint32_t)lane);
       uint32_t word[sizeof(v) / 4];
       memcpy(word, &v, sizeof(v));
 #pragma unroll
       for (int i = 0; i < (int)sizeof(v) / 4; ++i)
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at + 4 * i), "r"(word[i]) : "memory");
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there + 4 * i), "r"(word[i]) : "memory");
     }
   };
   auto told = [&] {
@@ -393,49 +412,59 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
     else __syncthreads();
   };
   if (stats) {
-    const uint4* at = (const uint4*)dyn + tid;
-    float m = -INFINITY, b = base_of(m, a.c);
-    float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
-    const float2 c2 = make_float2(a.c, a.c);
-    auto take = [&](auto pieces_now, int k) {
-      constexpr int P = decltype(pieces_now)::value;
-      float2 x[P][EI / 2];
-      float mx = -INFINITY;
+    const uint32_t none = minus_inf_word((const TI*)nullptr);
+    if (owner) {
+      float m = -INFINITY, b = base_of(m, a.c);
+      float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
+      const float2 c2 = make_float2(a.c, a.c);
+      auto take = [&](const uint4 (&u)[U]) {
+        float2 x[U][EI / 2];
+        float mx = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < P; ++j) {
-        unpack(at[(k + j) * NT], x[j], (const TI*)nullptr);
+        for (int j = 0; j < U; ++j) {
+          unpack(u[j], x[j], (const TI*)nullptr);
 #pragma unroll
-        for (int i = 0; i < EI / 2; ++i) mx = tc::fmax3(mx, x[j][i].x, x[j][i].y);
-      }
-      if (mx > m) {
-        const float nb = base_of(mx, a.c), f = tc::fast_exp2(b - nb);
-        s0 = tc::fmul2(s0, make_float2(f, f));
-        s1 = tc::fmul2(s1, make_float2(f, f));
-        m = mx;
-        b = nb;
-      }
-      const float2 nb = make_float2(-b, -b);
-#pragma unroll
-      for (int j = 0; j < P; ++j)
-#pragma unroll
-        for (int i = 0; i < EI / 2; ++i) {
-          const float2 t = tc::ffma2(x[j][i], c2, nb);
-          const float2 e = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
-          if (i & 1) s1 = tc::fadd2(s1, e);
-          else s0 = tc::fadd2(s0, e);
+          for (int i = 0; i < EI / 2; ++i) mx = tc::fmax3(mx, x[j][i].x, x[j][i].y);
         }
-    };
-    int k = 0;
-    for (; k + U <= mine; k += U) {
-      // one copy group has at most U pieces, and group g none behind piece (g + 1) U
-      if (OP != kDistill) copy_wait(max(0, mine / U - 1 - k / U));
-      take(std::integral_constant<int, U>{}, k);
+        if (mx > m) {
+          const float nb = base_of(mx, a.c), f = tc::fast_exp2(b - nb);
+          s0 = tc::fmul2(s0, make_float2(f, f));
+          s1 = tc::fmul2(s1, make_float2(f, f));
+          m = mx;
+          b = nb;
+        }
+        const float2 nb = make_float2(-b, -b);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+          for (int i = 0; i < EI / 2; ++i) {
+            const float2 t = tc::ffma2(x[j][i], c2, nb);
+            const float2 e = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
+            if (i & 1) s1 = tc::fadd2(s1, e);
+            else s0 = tc::fadd2(s0, e);
+          }
+      };
+      int k = 0;
+      for (; k + U <= mine; k += U) {
+        // group g of the copies ends with piece (g + 1) U at the latest
+        if (OP != kDistill) copy_wait(max(0, mine / U - 1 - k / U));
+        uint4 u[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) u[j] = at[(k + j) * NT];
+        take(u);
+      }
+      if (OP != kDistill) copy_wait(0);
+      if (k < mine) {
+        uint4 u[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          u[j] = k + j < mine ? at[(k + j) * NT] : make_uint4(none, none, none, none);
+        take(u);
+      }
+      rest = warp_join({m, (s0.x + s0.y) + (s1.x + s1.y)}, a.c);
     }
-    if (OP != kDistill) copy_wait(0);
-    for (; k < mine; ++k) take(std::integral_constant<int, 1>{}, k);
-    rest = warp_join({m, (s0.x + s0.y) + (s1.x + s1.y)}, a.c);
     double qz = 0.0;
-    if (OP == kDistill && warp == NW - 1) {
+    if (!owner) {
       for (int k = lane; k < a.K; k += 32) {
         const int i = t_idx[k];
         if (i >= e_lo && i < e_hi && t_q[k] != 0.f) qz += (double)t_q[k] * (double)t_z[k];
@@ -453,8 +482,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
     }
     // every warp's to every CTA of the cluster, joined there in a fixed order
     if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    tell(&s_rest[rank * NW + warp], rest);
-    if (OP == kDistill && warp == NW - 1) {
+    if (owner) {
+      tell(&s_rest[rank * NW + warp], rest);
+    } else {
       tell(&s_listed[rank], make_float4(listed.m, listed.s, count, 0.f));
       tell(&s_qz[rank], qz);
     }
@@ -466,166 +496,174 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_vocab_row(const RowArgs a) {
     if (is_far(rest.m)) {
       const Form f = form_of(rest.m, a.c);
       float s = 0.f;
-      for (k = 0; k < mine; ++k) {
+      for (int k = 0; k < mine; ++k) {
         float2 x[EI / 2];
         unpack(at[k * NT], x, (const TI*)nullptr);
 #pragma unroll
         for (int i = 0; i < EI / 2; ++i)
           s += tc::fast_exp2(fmaf(x[i].x, f.c, -f.b)) + tc::fast_exp2(fmaf(x[i].y, f.c, -f.b));
       }
-      tell(&s_again[rank * NW + warp], warp_sum(s));
+      s = warp_sum(s);
+      if (owner) tell(&s_again[rank * NW + warp], s);
       told();
       s = lane < C * NW ? s_again[lane] : 0.f;
       if (C * NW > 32 && lane + 32 < C * NW) s += s_again[lane + 32];
       rest.s = warp_sum(s);
     }
     if (OP == kDistill) {
-      listed = {-INFINITY, 0.f};
+      MaxSum one = {-INFINITY, 0.f};
       count = 0.f;
-      for (int i = 0; i < C; ++i) {
-        listed = join(listed, {s_listed[i].x, s_listed[i].y}, a.c);
-        count += s_listed[i].z;
+      if (lane < C) {
+        one = {s_listed[lane].x, s_listed[lane].y};
+        count = s_listed[lane].z;
       }
+      listed.m = warp_max_redux(one.m);
+      listed.s = warp_sum(one.s * rescale(one.m, listed.m, a.c));
+      count = warp_sum(count);
     }
   }
 
-  // ---- the row's scalars: dz = c_out 2^(c z - b) + corrections, in the form
-  // of the maximum outside the list
+  // ---- the row's scalars, by every thread: dz = c_out 2^(c z - b) +
+  // corrections, in the form of the maximum outside the list
   Form f = form_of(rest.m, a.c), f_in = f;
   float c_in = 0.f, c_out = 0.f, hot = 0.f;
-  if (OP == kLogpBwd) {
-    const double g = (double)dlogp * a.inv_tau;
-    hot = (float)g;
+  if (OP == kLogp) {
+    if (tid == 0 && rank == 0) {
+      const double ls = log((double)rest.s), logp = above(za, rest.m, a.c, a.inv_tau) - ls;
+      a.logp[row] = (float)logp;
+      if (a.logp_lo) a.logp_lo[row] = (float)(logp - (double)(float)logp);
+      a.lse[row] = (float)(ls - above(0.f, rest.m, a.c, a.inv_tau));
+    }
+    return;
+  } else if (OP == kLogpBwd) {
+    hot = (float)((double)dlogp * a.inv_tau);
     if (stats) {
-      c_out = (float)(-g / (double)rest.s);
+      c_out = -hot / rest.s;
     } else {
       // 2^(c z - log2(e) lse): the whole part stays in the exponent
       const double l2 = (double)lse_in * kLog2e;
       f.b = (float)rint(l2);
       c_out = -hot * tc::fast_exp2((float)((double)f.b - l2));
     }
-  } else if (OP != kDistill) {
-    if (tid == 0) {
-      const double ls = log((double)rest.s), logp = above(za, rest.m, a.c, a.inv_tau) - ls;
-      if (OP == kPolicy) {
-        const double A = a.advantage[row], ratio = exp(logp - (double)a.old_logp[row]);
-        const double lo = 1.0 - a.clip_low, hi = 1.0 + a.clip_high;
-        const bool clipped = (A > 0.0 && ratio > hi) || (A < 0.0 && ratio < lo);
-        double l = clipped ? -(A > 0.0 ? hi : lo) * A : -ratio * A;
-        double d = clipped ? 0.0 : -A * ratio;
-        if (a.ref_logp) {
-          const double gap = (double)a.ref_logp[row] - logp, e = expm1(gap);
-          l += a.kl_coef * (e - gap);
-          d -= a.kl_coef * e;
-        }
-        if (rank == 0) a.row_loss[row] = (float)((double)w * l);
-        const double g = a.scale * (double)w * d * a.inv_tau;
-        s_coef[0] = (float)g;
-        s_coef[1] = (float)(-g / (double)rest.s);
-      }
-      if (rank == 0) {
-        if (a.logp) a.logp[row] = (float)logp;
-        if (OP == kLogp && a.logp_lo) a.logp_lo[row] = (float)(logp - (double)(float)logp);
-        if (OP == kLogp && a.lse) a.lse[row] = (float)(ls - above(0.f, rest.m, a.c, a.inv_tau));
-      }
+  } else if (OP == kPolicy) {
+    // differences of log-probabilities in double, powers of them in fp32
+    const double logp = above(za, rest.m, a.c, a.inv_tau) - ln(rest.s);
+    const float ratio = expf((float)(logp - (double)old_logp));
+    const float lo = (float)(1.0 - a.clip_low), hi = (float)(1.0 + a.clip_high);
+    const bool clipped = (adv > 0.f && ratio > hi) || (adv < 0.f && ratio < lo);
+    float l = clipped ? -(adv > 0.f ? hi : lo) * adv : -ratio * adv;
+    float d = clipped ? 0.f : -adv * ratio;
+    if (a.ref_logp) {
+      const float gap = (float)((double)ref_logp - logp), e = expm1f(gap);
+      l += (float)a.kl_coef * (e - gap);
+      d -= (float)a.kl_coef * e;
     }
-    if (OP == kLogp || !dz) return;
-    __syncthreads();
-    hot = s_coef[0];
-    c_out = s_coef[1];
+    if (tid == 0 && rank == 0) {
+      a.row_loss[row] = w * l;
+      a.logp[row] = (float)logp;
+    }
+    hot = (float)(a.scale * a.inv_tau) * (w * d);
+    c_out = -hot / rest.s;
   } else {
     const MaxSum all = join(rest, listed, a.c);
     f_in = form_of(all.m, a.c);
     // without an entry outside the list there is no class for the rest
-    const double q_sum = s_q[0], q_rest = count == (float)V ? 0.0 : s_q[2];
-    if (tid == 0) {
-      const double g = a.scale * (double)w / a.inv_tau, Q = q_sum + q_rest;
-      const double in = Q / (double)all.s;
-      s_coef[0] = (float)g;
-      s_coef[1] = (float)(g * in);
-      // outside the list relative to the largest logit there: the student's
-      // mass outside may be too small to be held relative to the row's
-      // largest (none at all: an infinite loss, and entries of probability 0)
-      s_coef[2] = rest.s == 0.f ? (all.s == 0.f ? NAN : 0.f)
-                                : (float)(g * (in * (double)rescale(rest.m, all.m, a.c) -
-                                               (q_rest > 0.0 ? q_rest / (double)rest.s : 0.0)));
+    const float q_sum = (float)s_q[0], q_rest = count == (float)V ? 0.f : (float)s_q[2];
+    hot = (float)(a.scale / a.inv_tau) * w;
+    c_in = hot * (q_sum + q_rest) / all.s;
+    // outside the list relative to the largest logit there: the student's
+    // mass outside may be too small to be held relative to the row's largest
+    // (none at all: an infinite loss, and entries of probability 0)
+    c_out = rest.s == 0.f ? (all.s == 0.f ? NAN : 0.f)
+                          : c_in * rescale(rest.m, all.m, a.c) -
+                                (q_rest > 0.f ? hot * q_rest / rest.s : 0.f);
+    if (!owner && rank == 0 && lane == 0) {
+      const double qs = s_q[0], ls_all = ln(all.s), ls_rest = ln(rest.s);
+      double qz = 0.0;
+      for (int i = 0; i < C; ++i) qz += s_qz[i];
+      // sum of q (z / tau - lse), as above() has it of one z
+      const double x = is_far(all.m) ? (qz - qs * (double)all.m) * a.inv_tau
+                                     : (qz * (double)a.c - qs * (double)f_in.b) * kLn2;
+      double l = s_q[1] - (x - qs * ls_all);
+      if (q_rest > 0.f)  // -log of the student's share outside the list
+        l += (double)q_rest * ((double)logf(q_rest) + (ls_all - above(0.f, all.m, a.c, a.inv_tau)) -
+                               (ls_rest - above(0.f, rest.m, a.c, a.inv_tau)));
+      a.row_loss[row] = (float)((double)w * l / (a.inv_tau * a.inv_tau));
     }
-    // the loss, by a warp that writes its part of the adjoint later
-    if (warp == NW - 1 && rank == 0) {
-      const double ls = log((double)(lane == 0 ? all.s : lane == 1 ? rest.s : (float)q_rest));
-      const double ls_all = __shfl_sync(0xffffffffu, ls, 0), ls_rest = __shfl_sync(0xffffffffu, ls, 1);
-      if (lane == 2) {
-        double qz_all = 0.0;
-        for (int i = 0; i < C; ++i) qz_all += s_qz[i];
-        // sum of q (z / tau - lse), as above() has it of one z
-        const double x = is_far(all.m) ? (qz_all - q_sum * (double)all.m) * a.inv_tau
-                                       : (qz_all * (double)a.c - q_sum * (double)f_in.b) * kLn2;
-        double l = s_q[1] - (x - q_sum * ls_all);
-        if (q_rest > 0.0)  // -log of the student's share outside the list
-          l += q_rest * (ls + (ls_all - above(0.f, all.m, a.c, a.inv_tau)) -
-                         (ls_rest - above(0.f, rest.m, a.c, a.inv_tau)));
-        a.row_loss[row] = (float)((double)w * l / (a.inv_tau * a.inv_tau));
-      }
-    }
-    if (!dz) return;
-    __syncthreads();
-    hot = s_coef[0];
-    c_in = s_coef[1];
-    c_out = s_coef[2];
   }
+  if (!dz) return;
 
-  // ---- the adjoint, in 16-byte units of dz; an image whose pieces do not
-  // line up with them is read element by element
-  if (OP == kLogpBwd) {
-    copy_wait(0);
-    __syncthreads();
-  }
+  // ---- the adjoint
+  if (OP == kLogpBwd && !stats) copy_wait(0);
   const float2 c2 = make_float2(f.c, f.c), nb = make_float2(-f.b, -f.b);
   const float2 g2 = make_float2(c_out, c_out);
-  const int first = u0 + tid, at0 = first * EO - dph - e_org;
-  TO* out = dz + (first * EO - dph);
-  int to_token = token - (first * EO - dph);
-  auto units = [&](auto lined_up) {
-    const TI* in = image + at0;
-#pragma unroll 2
-    for (int u = first; u < u1; u += NT) {
-      float2 x[EO / 2];
-      if constexpr (decltype(lined_up)::value) {
+  auto values = [&](const float2 (&x)[EI / 2], float (&v)[EI], int e) {  // v[0] is element e's
 #pragma unroll
-        for (int k = 0; k < EO / EI; ++k)
-          unpack(((const uint4*)in)[k], &x[k * (EI / 2)], (const TI*)nullptr);
-      } else {
+    for (int i = 0; i < EI / 2; ++i) {
+      const float2 t = tc::ffma2(x[i], c2, nb);
+      const float2 d = tc::fmul2(make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y)), g2);
+      v[2 * i] = d.x;
+      v[2 * i + 1] = d.y;
+    }
+    const unsigned to = (unsigned)(token - e);
+    if (OP != kDistill && to < (unsigned)EI) {
 #pragma unroll
-        for (int k = 0; k < EO / 2; ++k) x[k] = make_float2(ld(&in[2 * k]), ld(&in[2 * k + 1]));
-      }
-      float v[EO];
-#pragma unroll
-      for (int k = 0; k < EO / 2; ++k) {
-        const float2 t = tc::ffma2(x[k], c2, nb);
-        const float2 d = tc::fmul2(make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y)), g2);
-        v[2 * k] = d.x;
-        v[2 * k + 1] = d.y;
-      }
-      if (OP != kDistill && (unsigned)to_token < (unsigned)EO) {
-#pragma unroll
-        for (int k = 0; k < EO; ++k)
-          if (to_token == k) v[k] += hot;
-      }
-      store_unit(out, v);
-      in += NT * EO;
-      out += NT * EO;
-      to_token -= NT * EO;
+      for (int i = 0; i < EI; ++i)
+        if (to == (unsigned)i) v[i] += hot;
     }
   };
-  if ((u0 * EO - dph - e_org) % EI == 0) units(std::true_type{});
-  else units(std::false_type{});
-  ragged([&](int e) {
-    const float d = c_out * tc::fast_exp2(fmaf(ld(&image[e - e_org]), f.c, -f.b));
-    st(&dz[e], OP != kDistill && e == token ? d + hot : d);
-  });
+  if ((uintptr_t)(dz + e_org) % (EI * sizeof(TO)) == 0) {
+    // the pieces' places in dz are aligned: every thread its own pieces
+    const int k0 = tid < f0 ? 1 : 0, k1 = owner && tid < f1 ? (f1 - tid + NT - 1) / NT : 0;
+#pragma unroll 2
+    for (int k = k0; k < k1; ++k) {
+      const int e = e_org + (tid + k * NT) * EI;
+      float2 x[EI / 2];
+      float v[EI];
+      unpack(at[k * NT], x, (const TI*)nullptr);
+      values(x, v, e);
+      store_n(dz + e, v);
+    }
+    // the pieces in part outside the row
+    auto in_part = [&](int i) {
+      const int e = e_org + i * EI;
+      float2 x[EI / 2];
+      float v[EI];
+      unpack(((const uint4*)dyn)[i], x, (const TI*)nullptr);
+      values(x, v, e);
+#pragma unroll
+      for (int j = 0; j < EI; ++j)
+        if (e + j >= 0 && e + j < V) st(&dz[e + j], v[j]);
+    };
+    if (f0 == 1 && tid == 0 && np > 0) in_part(0);
+    if (f1 < np && f1 >= f0 && tid == f1 % NT) in_part(f1);
+  } else {
+    // units of dz straddle pieces: read across them
+    __syncthreads();
+    const int dph = (int)((uintptr_t)dz % (EI * sizeof(TO))) / (int)sizeof(TO);
+    const int u0 = (dph + e_lo + EI - 1) / EI, u1 = (dph + e_hi) / EI;
+#pragma unroll 2
+    for (int u = u0 + tid; u < u1; u += kThreadsOf<OP>) {
+      const int e = u * EI - dph;
+      const TI* in = image + (e - e_org);
+      float2 x[EI / 2];
+      float v[EI];
+#pragma unroll
+      for (int i = 0; i < EI / 2; ++i) x[i] = make_float2(ld(&in[2 * i]), ld(&in[2 * i + 1]));
+      values(x, v, e);
+      store_n(dz + e, v);
+    }
+    const int ahead = u0 < u1 ? u0 * EI - dph : e_hi, behind = u0 < u1 ? u1 * EI - dph : e_hi;
+    auto one = [&](int e) {
+      const float d = c_out * tc::fast_exp2(fmaf(ld(&image[e - e_org]), f.c, -f.b));
+      st(&dz[e], OP != kDistill && e == token ? d + hot : d);
+    };
+    if (e_lo + tid < ahead) one(e_lo + tid);
+    if (behind + tid < e_hi) one(behind + tid);
+  }
   if (OP == kDistill) {
     __syncthreads();
-    for (int k = tid; k < a.K; k += NT)
+    for (int k = tid; k < a.K; k += kThreadsOf<OP>)
       if (!(t_g[k] < 0.f))
         st(&dz[t_idx[k]], c_in * tc::fast_exp2(fmaf(t_z[k], f_in.c, -f_in.b)) - hot * t_g[k]);
   }
@@ -701,6 +739,10 @@ __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_co
 }
 
 // ------------------------------------------------------------------- host
+// Shared memory of a list of K entries and its filter.
+constexpr int64_t list_bytes(int K) { return 16 * list_stride(K) + kFilterBits / 8; }
+constexpr int64_t kDynamicMost = kStageBytesMost + list_bytes(kMaxTeacherK);
+static_assert(kDynamicMost + 1536 <= 232448, "more shared memory than a CTA may have");
 // Let a kernel use the shared memory it may need, once per device.
 void allow_shared_memory(const void* kern) {
   static std::mutex mu;
@@ -710,20 +752,20 @@ void allow_shared_memory(const void* kern) {
   std::lock_guard<std::mutex> lock(mu);
   if (!done.count({dev, kern})) {
     DOP_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)(kStageBytesMost + 16 * kMaxTeacherK + kFilterBits / 8)));
+                                        (int)kDynamicMost));
     done.insert({dev, kern});
   }
 }
 
 // How the rows are laid out over CTAs: as few of them per row as hold its
-// 16-byte pieces in kStageBytes each, and at most kMaxCluster.
+// 16-byte pieces when three CTAs share an SM, and at most kMaxCluster.
 struct Split {
   int cluster, share;  // CTAs per row; pieces per CTA
 };
-Split split_of(int64_t rows, int64_t vocab, int prec) {
+Split split_of(int64_t rows, int64_t vocab, int prec, int64_t lists) {
   // the pieces that a row touches wherever it starts
   const int64_t size = prec == DOP_BF16 ? 2 : 4, pieces = ceil_div(vocab * size + 16 - size, 16);
-  const int64_t C = std::min<int64_t>(ceil_div(16 * pieces, kStageBytes), kMaxCluster);
+  const int64_t C = std::min<int64_t>(ceil_div(16 * pieces, kCtaBytes - lists), kMaxCluster);
   const int64_t share = ceil_div(pieces, C);
   if (16 * share > kStageBytesMost)
     throw Error(DOP_E_UNSUPPORTED, "vocab (" + std::to_string(vocab) + ") is above " +
@@ -735,18 +777,18 @@ Split split_of(int64_t rows, int64_t vocab, int prec) {
 template <RowOp OP>
 void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t s) {
   if (rows == 0) return;
-  const Split sp = split_of(rows, a.V, prec);
+  const int64_t lists = OP == kDistill ? list_bytes(a.K) : 0;
+  const Split sp = split_of(rows, a.V, prec, lists);
   a.cluster = sp.cluster;
   a.share = sp.share;
   a.stage_bytes = 16 * sp.share;
-  const size_t smem = (size_t)a.stage_bytes + (OP == kDistill ? 16 * (size_t)a.K + kFilterBits / 8 : 0);
   auto go = [&](auto ti, auto to) {
     auto kern = k_vocab_row<OP, decltype(ti), decltype(to)>;
     allow_shared_memory((const void*)kern);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * a.cluster));
-    cfg.blockDim = dim3(kRowThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(kThreadsOf<OP>);
+    cfg.dynamicSmemBytes = (size_t)(a.stage_bytes + lists);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -768,7 +810,7 @@ void check_rows(int64_t rows, int64_t vocab, int prec, const void* z, int64_t ld
   DOP_REQUIRE(rows >= 0 && rows <= INT32_MAX, "rows must lie in [0, 2^31)");
   DOP_REQUIRE(vocab >= 1 && vocab <= INT32_MAX, "vocab must lie in [1, 2^31)");
   DOP_REQUIRE(prec == DOP_F32 || prec == DOP_BF16, "unknown precision");
-  split_of(rows, vocab, prec);
+  split_of(rows, vocab, prec, 0);
   DOP_REQUIRE(ld >= vocab, "the logits' row stride is smaller than vocab");
   DOP_REQUIRE(z || rows == 0, "null logits");
   DOP_REQUIRE((uintptr_t)z % elem_bytes(prec) == 0, "misaligned logits");
