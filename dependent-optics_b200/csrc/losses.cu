@@ -219,9 +219,10 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
   __shared__ int s_twice;
   const int C = a.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool owner = OP != kDistill || tid < NT;  // of pieces
-  const int rank = (int)tc::cluster_ctarank();
-  uint32_t row32;
-  asm("mov.u32 %0, %%clusterid.x;" : "=r"(row32));
+  // (the log-probability's adjoint has nothing to exchange: plain CTAs)
+  const int rank = OP == kLogpBwd ? (int)(blockIdx.x % (unsigned)C) : (int)tc::cluster_ctarank();
+  uint32_t row32 = blockIdx.x / (unsigned)C;
+  if (OP != kLogpBwd) asm("mov.u32 %0, %%clusterid.x;" : "=r"(row32));
   const int64_t row = row32;
   const float w = a.weight ? a.weight[row] : 1.f;
   const int64_t token64 = OP == kDistill ? -1 : a.tokens[row];
@@ -230,6 +231,13 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
   const float adv = OP == kPolicy ? a.advantage[row] : 0.f;
   const float old_logp = OP == kPolicy ? a.old_logp[row] : 0.f;
   const float ref_logp = OP == kPolicy && a.ref_logp ? a.ref_logp[row] : 0.f;
+
+  int32_t my_idx = -1;
+  float my_top = 0.f;
+  if (OP == kDistill && tid < NT && tid < a.K) {
+    my_idx = a.top_index[row * a.K + tid];
+    my_top = a.top_logit[row * a.K + tid];
+  }
 
   const TI* z = (const TI*)a.z + row * a.ld;
   TO* dz = a.dz ? (TO*)a.dz + row * a.ldd : nullptr;
@@ -263,9 +271,7 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
     }
     return;
   }
-  // the log-probability's adjoint takes p from lse, but where fp32 does not
-  // hold lse to the digits that p needs
-  const bool stats = OP != kLogpBwd || fabsf(lse_in) > 256.f;
+  constexpr bool stats = OP != kLogpBwd;  // it has lse
   // every CTA of the cluster has started once this barrier is through: its
   // shared memory may be written to
   if (stats && C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -301,95 +307,96 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
   }
   const float za = OP == kDistill || OP == kLogpBwd ? 0.f : ld(&z[token]);
 
-  // ---- the teacher's list, by the warp that owns no pieces while the others
-  // wait for theirs: q, and which entries are a vocabulary entry's first
+  // ---- the teacher's list leaves the image.  While the copies run, the
+  // owners put the list into shared memory and find out whether an entry may
+  // be named twice (two entries on one bit of a filter); the warp that owns
+  // no pieces works out q while the others take the maximum and sum.
   const int K4 = OP == kDistill ? list_stride(a.K) : 0;
   int32_t* t_idx = (int32_t*)(dyn + a.stage_bytes);
-  float* t_q = (float*)t_idx + K4;  // q
+  float* t_q = (float*)t_idx + K4;  // the teacher's logit, then q
   float* t_z = t_q + K4;            // the student's logit, of this CTA's entries
   float* t_g = t_z + K4;            // this CTA's first ones: sum of q of the entry; else -1
   if (OP == kDistill) {
-    if (!owner) {
-      uint32_t* filter = (uint32_t*)(t_g + K4);
-      const int32_t* index = a.top_index + row * a.K;
-      const float* top = a.top_logit + row * a.K;
-      const double tl_given = a.teacher_lse ? (double)a.teacher_lse[row] : 0.0;
-      for (int i = lane; i < kFilterBits / 128; i += 32) ((uint4*)filter)[i] = make_uint4(0u, 0u, 0u, 0u);
-      MaxSum t = {-INFINITY, 0.f};
-      for (int k = lane; k < a.K; k += 32) {
-        const int32_t i = index[k];
-        const float y = top[k];
+    uint32_t* filter = (uint32_t*)(t_g + K4);
+    if (owner) {
+      for (int i = tid; i < kFilterBits / 128; i += NT) ((uint4*)filter)[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (tid == 0) s_twice = 0;
+      asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
+      for (int k = tid; k < a.K; k += NT) {
+        const int32_t i = k < NT ? my_idx : a.top_index[row * a.K + k];
+        const float y = k < NT ? my_top : a.top_logit[row * a.K + k];
         const bool in = i >= 0 && i < V;
         t_idx[k] = in ? i : -1;
         t_q[k] = in ? y : -INFINITY;
-        if (in) t.m = fmaxf(t.m, y);
-      }
-      __syncwarp();
-      // two entries on one bit: the list is compared entry by entry
-      bool twice = false;
-      for (int k = lane; k < a.K; k += 32)
-        if (t_idx[k] >= 0) {
-          const uint32_t h = (uint32_t)t_idx[k] % kFilterBits, bit = 1u << (h & 31);
-          if (atomicOr(&filter[h >> 5], bit) & bit) twice = true;
+        if (in) {
+          const uint32_t h = (uint32_t)i % kFilterBits, bit = 1u << (h & 31);
+          if (atomicOr(&filter[h >> 5], bit) & bit) s_twice = 1;
         }
-      twice = __any_sync(0xffffffffu, twice);
-      double tl = tl_given;
-      if (!a.teacher_lse) {
-        t.m = warp_max_redux(t.m);
-        const Form f = form_of(t.m, a.c);
-        for (int k = lane; k < a.K; k += 32) t.s += tc::fast_exp2(fmaf(t_q[k], f.c, -f.b));
-        tl = ln(warp_sum(t.s));
-      }
-      double qs = 0.0, ql = 0.0;
-      for (int k = lane; k < a.K; k += 32) {
-        const float y = t_q[k];
-        const double lq = (a.teacher_lse ? (double)y * a.inv_tau : above(y, t.m, a.c, a.inv_tau)) - tl;
-        const float hi = (float)lq;  // q to fp32's last digits: lq rounded, the rest applied
-        const float q = y == -INFINITY ? 0.f : expf(hi) * (1.f + (float)(lq - (double)hi));
-        const bool here = t_idx[k] >= e_lo && t_idx[k] < e_hi;
-        t_q[k] = q;
-        t_g[k] = here ? q : -1.f;
-        qs += (double)q;
-        if (q > 0.f) ql += (double)q * lq;
-      }
-      qs = warp_sum_d(qs);
-      ql = warp_sum_d(ql);
-      __syncwarp();
-      if (twice)
-        for (int k = lane; k < a.K; k += 32) {
-          const int i = t_idx[k];
-          if (t_g[k] < 0.f) continue;
-          double sum = 0.0;
-          bool first = true;
-          for (int j = 0; j < a.K; ++j)
-            if (t_idx[j] == i) {
-              if (j < k) first = false;
-              sum += (double)t_q[j];
-            }
-          t_g[k] = first ? (float)sum : -1.f;
-        }
-      if (lane == 0) {
-        s_q[0] = qs;
-        s_q[1] = ql;
-        s_q[2] = a.teacher_lse ? fmax(0.0, 1.0 - qs) : 0.0;
-        s_twice = twice;
       }
     }
-    // this CTA's entries leave the image
     copy_wait(0);
     __syncthreads();
     for (int k = tid; k < a.K; k += kThreadsOf<OP>) {
-      const bool here = t_idx[k] >= e_lo && t_idx[k] < e_hi;
-      t_z[k] = here ? ld(&image[t_idx[k] - e_org]) : 0.f;
-      if (!s_twice && here) image[t_idx[k] - e_org] = (TI)-INFINITY;
+      const int i = t_idx[k];
+      const bool here = i >= e_lo && i < e_hi;
+      t_z[k] = here ? ld(&image[i - e_org]) : 0.f;
+      t_g[k] = here ? 0.f : -1.f;
+      if (!s_twice && here) image[i - e_org] = (TI)-INFINITY;
     }
     __syncthreads();
     if (s_twice) {
       for (int k = tid; k < a.K; k += kThreadsOf<OP>)
-        if (!(t_g[k] < 0.f)) image[t_idx[k] - e_org] = (TI)-INFINITY;
+        if (t_g[k] == 0.f) image[t_idx[k] - e_org] = (TI)-INFINITY;
       __syncthreads();
     }
   }
+  // q of the list, its sums, and which entries are a vocabulary entry's first
+  auto make_q = [&] {
+    MaxSum t = {-INFINITY, 0.f};
+    double tl = 0.0;
+    if (a.teacher_lse) {
+      tl = (double)a.teacher_lse[row];
+    } else {
+      for (int k = lane; k < a.K; k += 32) t.m = fmaxf(t.m, t_q[k]);
+      t.m = warp_max_redux(t.m);
+      const Form f = form_of(t.m, a.c);
+      for (int k = lane; k < a.K; k += 32) t.s += tc::fast_exp2(fmaf(t_q[k], f.c, -f.b));
+      tl = ln(warp_sum(t.s));
+    }
+    double qs = 0.0, ql = 0.0;
+    for (int k = lane; k < a.K; k += 32) {
+      const float y = t_q[k];
+      const double lq = (a.teacher_lse ? (double)y * a.inv_tau : above(y, t.m, a.c, a.inv_tau)) - tl;
+      const float hi = (float)lq;  // q to fp32's last digits: lq rounded, the rest applied
+      const float q = y == -INFINITY ? 0.f : expf(hi) * (1.f + (float)(lq - (double)hi));
+      t_q[k] = q;
+      if (t_g[k] == 0.f) t_g[k] = q;
+      qs += (double)q;
+      if (q > 0.f) ql += (double)q * lq;
+    }
+    qs = warp_sum_d(qs);
+    ql = warp_sum_d(ql);
+    __syncwarp();
+    if (s_twice)
+      for (int k = lane; k < a.K; k += 32) {
+        const int i = t_idx[k];
+        if (t_g[k] < 0.f) continue;
+        double sum = 0.0;
+        bool first = true;
+        for (int j = 0; j < a.K; ++j)
+          if (t_idx[j] == i) {
+            if (j < k) first = false;
+            sum += (double)t_q[j];
+          }
+        t_g[k] = first ? (float)sum : -1.f;
+      }
+    __syncwarp();
+    if (lane == 0) {
+      s_q[0] = qs;
+      s_q[1] = ql;
+      s_q[2] = a.teacher_lse ? fmax(0.0, 1.0 - qs) : 0.0;
+    }
+  };
 
   // ---- maximum and sum
   MaxSum rest = {-INFINITY, 0.f}, listed = {-INFINITY, 0.f};
@@ -411,7 +418,7 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
     if (C > 1) tc::cluster_sync();
     else __syncthreads();
   };
-  if (stats) {
+  if constexpr (stats) {
     const uint32_t none = minus_inf_word((const TI*)nullptr);
     if (owner) {
       float m = -INFINITY, b = base_of(m, a.c);
@@ -465,6 +472,7 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
     }
     double qz = 0.0;
     if (!owner) {
+      make_q();
       for (int k = lane; k < a.K; k += 32) {
         const int i = t_idx[k];
         if (i >= e_lo && i < e_hi && t_q[k] != 0.f) qz += (double)t_q[k] * (double)t_z[k];
@@ -536,13 +544,15 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
     }
     return;
   } else if (OP == kLogpBwd) {
+    // 2^(c z - log2(e) lse): the whole part stays in the exponent.  An lse
+    // beyond 1e25 says nothing of p: 0
+    const double l2 = (double)lse_in * kLog2e;
     hot = (float)((double)dlogp * a.inv_tau);
-    if (stats) {
-      c_out = -hot / rest.s;
+    if (fabsf(lse_in) > 1e25f) {
+      f = {0.f, 1e4f};
+      c_out = -hot;
     } else {
-      // 2^(c z - log2(e) lse): the whole part stays in the exponent
-      const double l2 = (double)lse_in * kLog2e;
-      f.b = (float)rint(l2);
+      f = {a.c, (float)rint(l2)};
       c_out = -hot * tc::fast_exp2((float)((double)f.b - l2));
     }
   } else if (OP == kPolicy) {
@@ -594,7 +604,7 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
   if (!dz) return;
 
   // ---- the adjoint
-  if (OP == kLogpBwd && !stats) copy_wait(0);
+  if (OP == kLogpBwd) copy_wait(0);
   const float2 c2 = make_float2(f.c, f.c), nb = make_float2(-f.b, -f.b);
   const float2 g2 = make_float2(c_out, c_out);
   auto values = [&](const float2 (&x)[EI / 2], float (&v)[EI], int e) {  // v[0] is element e's
@@ -792,7 +802,7 @@ void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t 
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)a.cluster;
+    at[0].val.clusterDim.x = OP == kLogpBwd ? 1u : (unsigned)a.cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;

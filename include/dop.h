@@ -335,7 +335,8 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  *
  * Token log-probabilities: logp[r] = x[tokens[r]] - lse[r]; both are 0 for a
  * skipped row.  Backward: dlogits = dlogp / temperature ([v = token] - p), from
- * the lse of the forward; rows with dlogp 0 or a token outside [0, vocab) are
+ * the lse of the forward, whose rounding to fp32 p carries (2^-24 |lse|; beyond
+ * 1e25 p is taken as 0); rows with dlogp 0 or a token outside [0, vocab) are
  * skipped. */
 int dop_token_logp(int64_t rows, int64_t vocab, int precision, const void* logits, int64_t ld,
                    const int64_t* tokens, const float* weight, double temperature,
