@@ -24,10 +24,15 @@ call does not wait for it.  Arguments that do not fit raise DopError.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Any, NamedTuple
 
+import torch
+
 from ._lib import DOP_BF16, DOP_F32, DopError, check, lib
+
+_PRECISION = {torch.float32: DOP_F32, torch.bfloat16: DOP_BF16}
 
 
 class PolicyLoss(NamedTuple):
@@ -59,65 +64,56 @@ def _refuse(msg):
 
 def _matrix(t, name):
     """(rows, vocab, precision, row stride) of a matrix of logits."""
-    import torch
     if not isinstance(t, torch.Tensor) or t.dim() != 2 or not t.is_cuda:
         _refuse(f"{name} must be a CUDA tensor [rows, vocab]")
-    if t.dtype is torch.float32:
-        prec = DOP_F32
-    elif t.dtype is torch.bfloat16:
-        prec = DOP_BF16
-    else:
+    prec = _PRECISION.get(t.dtype)
+    if prec is None:
         _refuse(f"{name} must be float32 or bfloat16, not {t.dtype}")
     rows, vocab = t.shape
-    if vocab > 1 and t.stride(1) != 1:
+    ld, one = t.stride()
+    if one != 1 and vocab > 1:
         _refuse(f"the elements of a row of {name} must be contiguous")
-    return rows, vocab, prec, t.stride(0) if rows > 1 else max(t.stride(0), vocab)
+    return rows, vocab, prec, ld if rows > 1 else max(ld, vocab)
 
 
 def _vector(t, name, dtype, shape, device):
     """Device pointer of a contiguous tensor of that type and shape (None: NULL)."""
-    import torch
     if t is None:
         return None
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape:
-        _refuse(f"{name} must be a {dtype} tensor of shape {tuple(shape)}")
+        _refuse(f"{name} must be a {dtype} tensor of shape {shape}")
     if t.device != device or not t.is_contiguous():
         _refuse(f"{name} must be contiguous and on the logits' device")
     return t.data_ptr()
 
 
-class _On:
-    """The device of the logits and the stream of the call made current; what
-    the call allocates then belongs to that stream."""
+_HERE = contextlib.nullcontext()
 
-    def __init__(self, logits, stream):
-        import torch
-        self.ctx = None
-        if stream is not None:
-            if stream.device != logits.device:
-                _refuse("the stream belongs to another device than the logits")
-            self.ctx = torch.cuda.stream(stream)
-        elif logits.device.index != torch.cuda.current_device():
-            self.ctx = torch.cuda.device(logits.device)
 
-    def __enter__(self):
-        import torch
-        if self.ctx is not None:
-            self.ctx.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+def _on(logits, stream):
+    """A context in which the logits' device and the call's stream are current
+    (what the call allocates then belongs to that stream)."""
+    if stream is not None:
+        if stream.device != logits.device:
+            _refuse("the stream belongs to another device than the logits")
+        return torch.cuda.stream(stream)
+    if logits.get_device() != torch.cuda.current_device():
+        return torch.cuda.device(logits.device)
+    return _HERE
 
-    def __exit__(self, *a):
-        if self.ctx is not None:
-            self.ctx.__exit__(*a)
+
+def _current(device):
+    """The current stream's handle (without a Stream object: a microsecond of
+    a small call's time)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _gradient(logits, dlogits, grad_dtype, grad):
-    """dlogits (given, new, or None), its precision and row stride."""
-    import torch
+    """dlogits (given, new, or None), its pointer, precision and row stride."""
     if not grad:
         if dlogits is not None:
             _refuse("dlogits given although grad is False")
-        return None, DOP_F32, logits.shape[1]
+        return None, None, DOP_F32, logits.shape[1]
     if dlogits is None:
         dlogits = torch.empty(logits.shape, dtype=grad_dtype or logits.dtype, device=logits.device)
     elif dlogits.shape != logits.shape or dlogits.device != logits.device:
@@ -125,26 +121,21 @@ def _gradient(logits, dlogits, grad_dtype, grad):
     elif grad_dtype is not None and dlogits.dtype is not grad_dtype:
         _refuse("dlogits is not of grad_dtype")
     _, _, prec, ld = _matrix(dlogits, "dlogits")
-    return dlogits, prec, ld
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return dlogits, dlogits.data_ptr(), prec, ld
 
 
 def token_logp(logits, tokens, *, weight=None, temperature=1.0, stream=None):
     """(logp, lse), both float32 [rows]: the log-probability of tokens[r] under
     softmax(logits[r] / temperature), and the row's log-sum-exp."""
-    import torch
     rows, vocab, prec, ld = _matrix(logits, "logits")
     dev = logits.device
     tok = _vector(tokens, "tokens", torch.int64, (rows,), dev)
     w = _vector(weight, "weight", torch.float32, (rows,), dev)
-    with _On(logits, stream) as s:
+    with _on(logits, stream):
         logp = torch.empty(rows, dtype=torch.float32, device=dev)
-        lse = torch.empty(rows, dtype=torch.float32, device=dev)
+        lse = torch.empty_like(logp)
         check(lib().dop_token_logp(rows, vocab, prec, logits.data_ptr(), ld, tok, w, temperature,
-                                   logp.data_ptr(), lse.data_ptr(), s))
+                                   logp.data_ptr(), lse.data_ptr(), _current(dev)))
     return logp, lse
 
 
@@ -152,16 +143,15 @@ def token_logp_backward(logits, tokens, lse, dlogp, *, temperature=1.0, dlogits=
                         grad_dtype=None, stream=None):
     """dlogits from dlogp [rows], the adjoint of `token_logp`'s logp, and the
     lse it returned.  Rows with dlogp 0 get a row of zeros."""
-    import torch
     rows, vocab, prec, ld = _matrix(logits, "logits")
     dev = logits.device
     tok = _vector(tokens, "tokens", torch.int64, (rows,), dev)
     l = _vector(lse, "lse", torch.float32, (rows,), dev)
     g = _vector(dlogp, "dlogp", torch.float32, (rows,), dev)
-    with _On(logits, stream) as s:
-        dlogits, gprec, ldd = _gradient(logits, dlogits, grad_dtype, True)
+    with _on(logits, stream):
+        dlogits, dz, gprec, ldd = _gradient(logits, dlogits, grad_dtype, True)
         check(lib().dop_token_logp_backward(rows, vocab, prec, logits.data_ptr(), ld, tok, l, g,
-                                            temperature, gprec, dlogits.data_ptr(), ldd, s))
+                                            temperature, gprec, dz, ldd, _current(dev)))
     return dlogits
 
 
@@ -170,7 +160,6 @@ def policy_loss(logits, tokens, old_logp, advantage, *, ref_logp=None, weight=No
                 dlogits=None, grad_dtype=None, grad=True, stream=None) -> PolicyLoss:
     """The clipped policy loss with a KL term towards ref_logp; `scale`
     defaults to 1 / rows."""
-    import torch
     rows, vocab, prec, ld = _matrix(logits, "logits")
     dev, f32, one = logits.device, torch.float32, (rows,)
     tok = _vector(tokens, "tokens", torch.int64, one, dev)
@@ -180,15 +169,15 @@ def policy_loss(logits, tokens, old_logp, advantage, *, ref_logp=None, weight=No
     w = _vector(weight, "weight", f32, one, dev)
     if scale is None:
         scale = 1.0 / max(rows, 1)
-    with _On(logits, stream) as s:
+    with _on(logits, stream):
         loss = torch.empty((), dtype=f32, device=dev)
         row_loss = torch.empty(rows, dtype=f32, device=dev)
-        logp = torch.empty(rows, dtype=f32, device=dev)
-        dlogits, gprec, ldd = _gradient(logits, dlogits, grad_dtype, grad)
+        logp = torch.empty_like(row_loss)
+        dlogits, dz, gprec, ldd = _gradient(logits, dlogits, grad_dtype, grad)
         check(lib().dop_policy_loss_grad(rows, vocab, prec, logits.data_ptr(), ld, tok, old, adv,
                                          ref, w, temperature, clip_low, clip_high, kl_coef, scale,
                                          loss.data_ptr(), row_loss.data_ptr(), logp.data_ptr(),
-                                         gprec, _ptr(dlogits), ldd, s))
+                                         gprec, dz, ldd, _current(dev)))
     return PolicyLoss(loss, row_loss, logp, dlogits)
 
 
@@ -200,7 +189,6 @@ def preference_loss(logits, tokens, seq_off, *, ref_logp=None, weight=None, temp
     row offsets: pair i's chosen sequence is rows seq_off[2i] .. seq_off[2i+1],
     its rejected one seq_off[2i+1] .. seq_off[2i+2].  `scale` defaults to
     1 / pairs."""
-    import torch
     rows, vocab, prec, ld = _matrix(logits, "logits")
     dev, f32, one = logits.device, torch.float32, (rows,)
     if isinstance(seq_off, torch.Tensor):
@@ -217,19 +205,19 @@ def preference_loss(logits, tokens, seq_off, *, ref_logp=None, weight=None, temp
     w = _vector(weight, "weight", f32, one, dev)
     if scale is None:
         scale = 1.0 / max(pairs, 1)
-    with _On(logits, stream) as s:
+    with _on(logits, stream):
         loss = torch.empty((), dtype=f32, device=dev)
         pair_loss = torch.empty(pairs, dtype=f32, device=dev)
-        margin = torch.empty(pairs, dtype=f32, device=dev)
+        margin = torch.empty_like(pair_loss)
         logp = torch.empty(rows, dtype=f32, device=dev)
-        lse = torch.empty(rows, dtype=f32, device=dev)
-        dlogp = torch.empty(rows, dtype=f32, device=dev)
-        dlogits, gprec, ldd = _gradient(logits, dlogits, grad_dtype, grad)
+        lse = torch.empty_like(logp)
+        dlogp = torch.empty_like(logp)
+        dlogits, dz, gprec, ldd = _gradient(logits, dlogits, grad_dtype, grad)
         check(lib().dop_preference_loss_grad(
             rows, vocab, prec, logits.data_ptr(), ld, tok, pairs, off, ref, w, temperature, beta,
             label_smoothing, int(length_normalize), scale, loss.data_ptr(), pair_loss.data_ptr(),
             margin.data_ptr(), logp.data_ptr(), lse.data_ptr(), dlogp.data_ptr(), gprec,
-            _ptr(dlogits), ldd, s))
+            dz, ldd, _current(dev)))
     return PreferenceLoss(loss, pair_loss, margin, logp, lse, dlogp, dlogits)
 
 
@@ -239,7 +227,6 @@ def distill_loss(logits, top_index, top_logit, *, teacher_lse=None, weight=None,
     float32, both [rows, top_k]); with `teacher_lse` [rows], the log-sum-exp of
     the teacher's whole row over the temperature, the mass outside the listed
     entries is one more class.  `scale` defaults to 1 / rows."""
-    import torch
     rows, vocab, prec, ld = _matrix(logits, "logits")
     dev, f32 = logits.device, torch.float32
     if not isinstance(top_index, torch.Tensor) or top_index.dim() != 2:
@@ -251,11 +238,11 @@ def distill_loss(logits, top_index, top_logit, *, teacher_lse=None, weight=None,
     w = _vector(weight, "weight", f32, (rows,), dev)
     if scale is None:
         scale = 1.0 / max(rows, 1)
-    with _On(logits, stream) as s:
+    with _on(logits, stream):
         loss = torch.empty((), dtype=f32, device=dev)
         row_loss = torch.empty(rows, dtype=f32, device=dev)
-        dlogits, gprec, ldd = _gradient(logits, dlogits, grad_dtype, grad)
+        dlogits, dz, gprec, ldd = _gradient(logits, dlogits, grad_dtype, grad)
         check(lib().dop_distill_loss_grad(rows, vocab, prec, logits.data_ptr(), ld, k, idx, top,
                                           tl, w, temperature, scale, loss.data_ptr(),
-                                          row_loss.data_ptr(), gprec, _ptr(dlogits), ldd, s))
+                                          row_loss.data_ptr(), gprec, dz, ldd, _current(dev)))
     return DistillLoss(loss, row_loss, dlogits)
