@@ -51,6 +51,10 @@ struct RowArgs {
   const float* weight;  // null: 1
   double inv_tau;
   float c;       // log2(e) / tau
+  int64_t rows, in_lo, in_hi;  // rows outside [in_lo, in_hi) are skipped
+  const float* sum_of;  // the preference loss: scale times the sum of these,
+  int64_t sum_n;        // taken with the adjoint
+  float* loss;
   int cluster;      // CTAs per row
   int share;        // 16-byte pieces of a row a CTA has
   int stage_bytes;  // of shared memory for a CTA's pieces
@@ -205,7 +209,7 @@ template <RowOp OP>
 constexpr int kThreadsOf = kRowThreads + (OP == kDistill ? 32 : 0);
 
 template <RowOp OP, typename TI, typename TO>
-__global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a) {
+__device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, const int rank) {
   constexpr int EI = 16 / (int)sizeof(TI);
   constexpr int NT = kRowThreads, NW = NT / 32, U = 4;
   extern __shared__ __align__(16) uint8_t dyn[];
@@ -219,11 +223,6 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
   __shared__ int s_twice;
   const int C = a.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool owner = OP != kDistill || tid < NT;  // of pieces
-  // (the log-probability's adjoint has nothing to exchange: plain CTAs)
-  const int rank = OP == kLogpBwd ? (int)(blockIdx.x % (unsigned)C) : (int)tc::cluster_ctarank();
-  uint32_t row32 = blockIdx.x / (unsigned)C;
-  if (OP != kLogpBwd) asm("mov.u32 %0, %%clusterid.x;" : "=r"(row32));
-  const int64_t row = row32;
   const float w = a.weight ? a.weight[row] : 1.f;
   const int64_t token64 = OP == kDistill ? -1 : a.tokens[row];
   const float dlogp = OP == kLogpBwd ? a.dlogp[row] : 0.f;
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
   // pieces that lie in the row altogether: [f0, f1)
   const int f0 = e_org < 0 ? 1 : 0, f1 = e_org + np * EI > V ? np - 1 : np;
 
-  if (w == 0.f || (OP != kDistill && (token64 < 0 || token64 >= V)) ||
+  if (w == 0.f || row < a.in_lo || row >= a.in_hi || (OP != kDistill && (token64 < 0 || token64 >= V)) ||
       (OP == kLogpBwd && dlogp == 0.f)) {
     if (dz) {
       constexpr int EO = 16 / (int)sizeof(TO);
@@ -679,27 +678,50 @@ __global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a
   }
 }
 
-// loss = scale * sum of l[0 .. n), in a fixed order.
-__global__ void __launch_bounds__(1024) k_scaled_sum(const float* __restrict__ l, int64_t n,
-                                                     double scale, float* __restrict__ loss) {
-  __shared__ double red[32];
+// loss = scale * sum of l[0 .. n), in a fixed order, by NT threads.
+template <int NT>
+__device__ __forceinline__ void scaled_sum_of(const float* l, int64_t n, double scale, float* loss) {
+  __shared__ double red[NT / 32];
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)l[i];
+  for (int64_t i = threadIdx.x; i < n; i += NT) s += (double)l[i];
   s = warp_sum_d(s);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     double t = 0.0;
-    for (int w = 0; w < 32; ++w) t += red[w];
+    for (int w = 0; w < NT / 32; ++w) t += red[w];
     *loss = (float)(scale * t);
   }
 }
+__global__ void __launch_bounds__(1024) k_scaled_sum(const float* l, int64_t n, double scale, float* loss) {
+  scaled_sum_of<1024>(l, n, scale, loss);
+}
 
-// One CTA per pair: rows [off[2p], off[2p+1]) chosen, [off[2p+1], off[2p+2])
-// rejected; the margin, the pair's loss, and each row's dlogp.  dlogp comes in
-// holding what the rounding of logp to fp32 left out: a margin is a small
-// difference of sums of log-probabilities, and would show it.
-constexpr int kPairsPerLaunch = 128;
+template <RowOp OP, typename TI, typename TO>
+__global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a) {
+  if (OP == kLogpBwd) {
+    // it has nothing to exchange: plain CTAs.  Last rows first: they are the
+    // ones that the log-probabilities' pass has left in L2
+    const unsigned C = (unsigned)a.cluster, r = blockIdx.x / C;
+    if (r == a.rows) return scaled_sum_of<kRowThreads>(a.sum_of, a.sum_n, a.scale, a.loss);
+    vocab_row<OP, TI, TO>(a, a.rows - 1 - r, (int)(blockIdx.x % C));
+  } else {
+    uint32_t row;
+    asm("mov.u32 %0, %%clusterid.x;" : "=r"(row));
+    vocab_row<OP, TI, TO>(a, row, (int)tc::cluster_ctarank());
+  }
+}
+
+// ---- the preference loss
+// A row's adjoint needs the margin of its pair, so the rows are read twice:
+// for their log-probabilities, then, after the margins, for the adjoint, last
+// rows first (what the first reading left in L2).
+//
+// A pair, by one CTA: rows [off[2p], off[2p+1]) chosen, [off[2p+1],
+// off[2p+2]) rejected; the margin, the pair's loss, and each row's dlogp.
+// dlogp comes in holding what the rounding of logp to fp32 left out: a margin
+// is a small difference of sums of log-probabilities, and would show it.
+constexpr int kPairsPerLaunch = 64;
 struct PairArgs {
   int64_t off[2 * kPairsPerLaunch + 1];
   int64_t V;
@@ -711,7 +733,8 @@ struct PairArgs {
 };
 __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_constant__ PairArgs a) {
   __shared__ double s_red[kRowThreads / 32];
-  const int64_t* off = a.off + 2 * blockIdx.x;
+  const int pair = blockIdx.x;
+  const int64_t* off = a.off + 2 * pair;
   auto weight_of = [&](int64_t t) {
     const int64_t k = a.tokens[t];
     return k < 0 || k >= a.V ? 0.f : (a.weight ? a.weight[t] : 1.f);
@@ -736,8 +759,8 @@ __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_co
   const double l = (1.0 - a.smoothing) * (fmax(-m, 0.0) + tail) + a.smoothing * (fmax(m, 0.0) + tail);
   const double dm = a.smoothing / (1.0 + exp(-m)) - (1.0 - a.smoothing) / (1.0 + exp(m));
   if (threadIdx.x == 0) {
-    a.pair_loss[blockIdx.x] = (float)l;
-    a.margin[blockIdx.x] = (float)m;
+    a.pair_loss[pair] = (float)l;
+    a.margin[pair] = (float)m;
   }
   for (int q = 0; q < 2; ++q) {
     const double g = (q ? -dm : dm) * a.beta * a.scale / (len[q] != 0.0 ? len[q] : 1.0);
@@ -780,8 +803,33 @@ Split split_of(int64_t rows, int64_t vocab, int prec, int64_t lists) {
   if (16 * share > kStageBytesMost)
     throw Error(DOP_E_UNSUPPORTED, "vocab (" + std::to_string(vocab) + ") is above " +
                                        std::to_string((C * kStageBytesMost - 16) / size + 1));
-  if (rows * C > INT32_MAX) throw Error(DOP_E_UNSUPPORTED, "too many rows for this vocab");
+  if (rows * C >= INT32_MAX) throw Error(DOP_E_UNSUPPORTED, "too many rows for this vocab");
   return {(int)C, (int)share};
+}
+
+// f(kernel's logit type, dlogits type)
+template <typename F>
+void by_types(int prec, int grad_prec, bool grad, F&& f) {
+  if (prec == DOP_BF16) f(bf16{}, bf16{});
+  else if (grad && grad_prec == DOP_BF16) f(0.f, bf16{});
+  else f(0.f, 0.f);
+}
+template <typename A>
+void launch(void (*kern)(A), const A& a, int64_t ctas, int threads, int64_t smem, int cluster,
+            cudaStream_t s) {
+  allow_shared_memory((const void*)kern);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  DOP_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
 template <RowOp OP>
@@ -792,25 +840,12 @@ void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t 
   a.cluster = sp.cluster;
   a.share = sp.share;
   a.stage_bytes = 16 * sp.share;
-  auto go = [&](auto ti, auto to) {
-    auto kern = k_vocab_row<OP, decltype(ti), decltype(to)>;
-    allow_shared_memory((const void*)kern);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * a.cluster));
-    cfg.blockDim = dim3(kThreadsOf<OP>);
-    cfg.dynamicSmemBytes = (size_t)(a.stage_bytes + lists);
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = OP == kLogpBwd ? 1u : (unsigned)a.cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    DOP_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
-  };
-  if (prec == DOP_BF16) go(bf16{}, bf16{});
-  else if (a.dz && grad_prec == DOP_BF16) go(0.f, bf16{});
-  else go(0.f, 0.f);
+  a.rows = rows;
+  const int64_t ctas = rows * a.cluster + (a.sum_of ? 1 : 0);
+  by_types(prec, grad_prec, a.dz != nullptr, [&](auto ti, auto to) {
+    launch(k_vocab_row<OP, decltype(ti), decltype(to)>, a, ctas, kThreadsOf<OP>,
+           a.stage_bytes + lists, OP == kLogpBwd ? 1 : a.cluster, s);
+  });
 }
 
 int elem_bytes(int prec) { return prec == DOP_BF16 ? 2 : 4; }
@@ -852,6 +887,8 @@ RowArgs row_args(int64_t vocab, const void* z, int64_t ld, const int64_t* tokens
   a.tokens = tokens;
   a.weight = weight;
   a.inv_tau = 1.0 / tau;
+  a.in_lo = 0;
+  a.in_hi = INT64_MAX;
   a.c = (float)(kLog2e / tau);
   return a;
 }
@@ -967,21 +1004,13 @@ int dop_preference_loss_grad(int64_t rows, int64_t vocab, int precision, const v
     DOP_REQUIRE(seq_off[2 * pairs] <= rows, "seq_off ends behind the last row");
     check_grad(rows, vocab, precision, logits, ld, grad_precision, dlogits, ldd);
     cudaStream_t s = as_stream(stream);
-    const int64_t a0 = seq_off[0], a1 = seq_off[2 * pairs];
-    const int zb = elem_bytes(precision);
-    // rows of no sequence
-    for (int64_t part = 0; part < 2; ++part) {
-      const int64_t lo = part ? a1 : 0, n = (part ? rows : a0) - lo;
-      if (n == 0) continue;
-      for (float* p : {logp, lse, dlogp})
-        DOP_CHECK_CUDA(cudaMemsetAsync(p + lo, 0, sizeof(float) * n, s));
-    }
-    RowArgs f = row_args(vocab, (const char*)logits + a0 * ld * zb, ld, tokens + a0,
-                         weight ? weight + a0 : nullptr, temperature);
-    f.logp = logp + a0;
-    f.lse = lse + a0;
-    f.logp_lo = dlogp + a0;
-    launch_rows<kLogp>(f, a1 - a0, precision, DOP_F32, s);
+    RowArgs f = row_args(vocab, logits, ld, tokens, weight, temperature);
+    f.in_lo = seq_off[0];
+    f.in_hi = seq_off[2 * pairs];
+    f.logp = logp;
+    f.logp_lo = dlogp;
+    f.lse = lse;
+    launch_rows<kLogp>(f, rows, precision, DOP_F32, s);
     for (int64_t p0 = 0; p0 < pairs; p0 += kPairsPerLaunch) {
       const int64_t n = std::min<int64_t>(pairs - p0, kPairsPerLaunch);
       PairArgs pa{};
@@ -1001,15 +1030,17 @@ int dop_preference_loss_grad(int64_t rows, int64_t vocab, int precision, const v
       k_preference_pair<<<(unsigned)n, kRowThreads, 0, s>>>(pa);
       DOP_CHECK_CUDA(cudaGetLastError());
     }
-    if (dlogits) {
-      RowArgs b = row_args(vocab, logits, ld, tokens, nullptr, temperature);
-      b.lse = lse;
-      b.dlogp = dlogp;
-      b.dz = dlogits;
-      b.ldd = ldd;
-      launch_rows<kLogpBwd>(b, rows, precision, grad_precision, s);
-    }
-    scaled_sum(pair_loss, pairs, scale, loss, s);
+    if (!dlogits || rows == 0) return scaled_sum(pair_loss, pairs, scale, loss, s);
+    RowArgs b = row_args(vocab, logits, ld, tokens, nullptr, temperature);
+    b.lse = lse;
+    b.dlogp = dlogp;
+    b.dz = dlogits;
+    b.ldd = ldd;
+    b.sum_of = pair_loss;
+    b.sum_n = pairs;
+    b.scale = scale;
+    b.loss = loss;
+    launch_rows<kLogpBwd>(b, rows, precision, grad_precision, s);
   });
 }
 
