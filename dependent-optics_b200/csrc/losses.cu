@@ -36,6 +36,8 @@ enum RowOp : int { kLogp = 0, kLogpBwd = 1, kPolicy = 2, kDistill = 3 };
 constexpr int kRowThreads = 256;
 constexpr int kMaxTeacherK = 1024;
 constexpr int kMaxCluster = 8;
+constexpr int kOnceThreads = 128, kOnceCtas = 8;
+constexpr int kRing = 8;  // pieces that a thread reading a row once has under way
 // Shared memory: of a CTA when three are to fit an SM (of its 228 KB, less the
 // static share and what the system takes of each), and of a CTA's pieces at most.
 constexpr int64_t kCtaBytes = 228 * 1024 / 3 - 2560, kStageBytesMost = 200 * 1024;
@@ -84,7 +86,8 @@ struct RowArgs {
 // far, and its powers are taken of (z - m) 2^-40, which is exact.
 constexpr float kFar = 1e30f;
 __device__ __forceinline__ float base_of(float m, float c) {
-  return fminf(fmaxf(rintf(c * m), -kFar), kFar);
+  constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: to a whole number without a conversion
+  return fminf(fmaxf((c * m + kRound) - kRound, -kFar), kFar);
 }
 __device__ __forceinline__ bool is_far(float m) { return fabsf(m) > 1e25f && m != -INFINITY; }
 struct Form {
@@ -206,16 +209,20 @@ __device__ __forceinline__ double ln(float s) {
 // A cluster of a.cluster CTAs per row: 256 threads own the pieces, and
 // distillation has a warp more for the teacher's list.
 template <RowOp OP>
-constexpr int kThreadsOf = kRowThreads + (OP == kDistill ? 32 : 0);
+constexpr int kOwnersOf = OP == kLogp ? kOnceThreads : kRowThreads;
+template <RowOp OP>
+constexpr int kThreadsOf = kOwnersOf<OP> + (OP == kDistill ? 32 : 0);
+template <RowOp OP>
+constexpr int kCtasPerSM = OP == kLogp ? kOnceCtas : 3;
 
 template <RowOp OP, typename TI, typename TO>
 __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, const int rank) {
   constexpr int EI = 16 / (int)sizeof(TI);
-  constexpr int NT = kRowThreads, NW = NT / 32, U = 4;
+  constexpr int NT = kOwnersOf<OP>, NW = NT / 32, U = OP == kLogp ? 2 : 4;
   extern __shared__ __align__(16) uint8_t dyn[];
   // of every warp of the cluster
   __shared__ MaxSum s_rest[kMaxCluster * NW];
-  __shared__ float s_again[kMaxCluster * NW];
+  __shared__ float s_again[2 * kMaxCluster * NW];
   // of every CTA: the listed entries' m, s, count; the sum of q times the logit
   __shared__ __align__(16) float4 s_listed[kMaxCluster];
   __shared__ double s_qz[kMaxCluster];
@@ -277,33 +284,53 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
 
   // ---- copy this CTA's pieces; a thread owns pieces tid + NT k, and the
   // first `mine` of them are the row's
+  // (the log-probability reads its pieces once, in a ring of kRing of them)
+  constexpr bool kOnce = OP == kLogp;
   TI* image = (TI*)dyn;
-  uint4* at = (uint4*)dyn + tid;  // piece k: at[k NT]
+  uint4* at = (uint4*)dyn + tid;  // piece k: at[k NT], in the ring at[(k % kRing) NT]
+  auto place = [&](int k) { return kOnce ? (k % kRing) * NT : k * NT; };
   const int mine = owner && tid < np ? (np - tid + NT - 1) / NT : 0;
-  if (owner) {
-    // the first and the last piece of the row may be in part outside it
-    auto in_part = [&](int i) {
+  // the first and the last piece of the row may be in part outside it
+  auto edge = [&](int i) {
+    TI v[EI];
 #pragma unroll
-      for (int k = 0; k < EI; ++k) {
-        const int e = e_org + i * EI + k;
-        image[i * EI + k] = e >= 0 && e < V ? z[e] : (TI)-INFINITY;
-      }
-    };
-    if (f0 == 1 && tid == 0 && np > 0) in_part(0);
-    if (f1 < np && f1 >= f0 && tid == f1 % NT) in_part(f1);
-    const int i0 = tid < f0 ? tid + NT : tid;
-    const uint32_t dst = tc::smem_u32(dyn) + i0 * 16;
-    const uint4* src = (const uint4*)(z + e_org) + i0;
-    const int n = i0 < f1 ? (f1 - i0 + NT - 1) / NT : 0;
+    for (int k = 0; k < EI; ++k) {
+      const int e = e_org + i * EI + k;
+      v[k] = e >= 0 && e < V ? z[e] : (TI)-INFINITY;
+    }
+    uint4 u;
+    memcpy(&u, v, 16);
+    return u;
+  };
+  const uint4* src = (const uint4*)(z + e_org) + tid;
+  const uint32_t dst = tc::smem_u32(at);
+  auto whole = [&](int k) { return tid + k * NT >= f0 && tid + k * NT < f1; };
+  auto copy_whole = [&](int k) {
+    if (whole(k)) copy_piece(dst + place(k) * 16, src + k * NT);
+  };
+  if (owner) {
+    const int n = kOnce ? min(mine, kRing) : mine;
     int k = 0;
     for (; k + U <= n; k += U) {
+      if (tid + k * NT >= f0 && tid + (k + U - 1) * NT < f1) {
 #pragma unroll
-      for (int j = 0; j < U; ++j) copy_piece(dst + (k + j) * (NT * 16), src + (k + j) * NT);
+        for (int j = 0; j < U; ++j) copy_piece(dst + place(k + j) * 16, src + (k + j) * NT);
+      } else {
+        for (int j = 0; j < U; ++j) copy_whole(k + j);
+      }
       copy_commit();
     }
-    for (; k < n; ++k) copy_piece(dst + k * (NT * 16), src + k * NT);
+    for (; k < n; ++k) copy_whole(k);
     copy_commit();
+    // the two that a row may share with what lies beside it, while the copies run
+    if (f0 == 1 && tid == 0 && n > 0) at[0] = edge(0);
+    if (f1 < np && f1 >= f0 && tid == f1 % NT && f1 / NT < n) at[place(f1 / NT)] = edge(f1);
   }
+  // piece k once more, after its copy (a ring may have given it up)
+  auto piece = [&](int k) {
+    const int i = tid + k * NT;
+    return !kOnce ? at[k * NT] : i >= f0 && i < f1 ? src[k * NT] : edge(i);
+  };
   const float za = OP == kDistill || OP == kLogpBwd ? 0.f : ld(&z[token]);
 
   // ---- the teacher's list leaves the image.  While the copies run, the
@@ -420,54 +447,78 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
   if constexpr (stats) {
     const uint32_t none = minus_inf_word((const TI*)nullptr);
     if (owner) {
-      float m = -INFINITY, b = base_of(m, a.c);
-      float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
+      // the sum is taken relative to the largest of the first pieces; should
+      // a later element pass that by 2^127, the sum says so and is taken
+      // again relative to the maximum of all
+      float m = -INFINITY;
+      float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f), nb = s0;
       const float2 c2 = make_float2(a.c, a.c);
-      auto take = [&](const uint4 (&u)[U]) {
-        float2 x[U][EI / 2];
-        float mx = -INFINITY;
+      auto largest = [&](uint4 u) {
+        float2 x[EI / 2];
+        unpack(u, x, (const TI*)nullptr);
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-          unpack(u[j], x[j], (const TI*)nullptr);
-#pragma unroll
-          for (int i = 0; i < EI / 2; ++i) mx = tc::fmax3(mx, x[j][i].x, x[j][i].y);
-        }
-        if (mx > m) {
-          const float nb = base_of(mx, a.c), f = tc::fast_exp2(b - nb);
-          s0 = tc::fmul2(s0, make_float2(f, f));
-          s1 = tc::fmul2(s1, make_float2(f, f));
-          m = mx;
-          b = nb;
-        }
-        const float2 nb = make_float2(-b, -b);
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-#pragma unroll
-          for (int i = 0; i < EI / 2; ++i) {
-            const float2 t = tc::ffma2(x[j][i], c2, nb);
-            const float2 e = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
-            if (i & 1) s1 = tc::fadd2(s1, e);
-            else s0 = tc::fadd2(s0, e);
-          }
+        for (int i = 0; i < EI / 2; ++i) m = tc::fmax3(m, x[i].x, x[i].y);
       };
+      auto add = [&](uint4 u) {
+        float2 x[EI / 2];
+        unpack(u, x, (const TI*)nullptr);
+#pragma unroll
+        for (int i = 0; i < EI / 2; ++i) {
+          const float2 t = tc::ffma2(x[i], c2, nb);
+          const float2 e = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
+          if (i & 1) s1 = tc::fadd2(s1, e);
+          else s0 = tc::fadd2(s0, e);
+        }
+      };
+      auto relative_to_m = [&] { nb.x = nb.y = -base_of(m, a.c); };
+      auto sum = [&] { return (s0.x + s0.y) + (s1.x + s1.y); };
       int k = 0;
       for (; k + U <= mine; k += U) {
-        // group g of the copies ends with piece (g + 1) U at the latest
-        if (OP != kDistill) copy_wait(max(0, mine / U - 1 - k / U));
+        // group g of the copies ends with piece (g + 1) U at the latest; a
+        // ring keeps kRing / U groups under way
+        if (kOnce) copy_wait(mine > kRing ? kRing / U - 1 : max(0, mine / U - 1 - k / U));
+        else if (OP != kDistill) copy_wait(max(0, mine / U - 1 - k / U));
         uint4 u[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) u[j] = at[(k + j) * NT];
-        take(u);
+        for (int j = 0; j < U; ++j) u[j] = at[place(k + j)];
+        if (k == 0) {
+#pragma unroll
+          for (int j = 0; j < U; ++j) largest(u[j]);
+          relative_to_m();
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) add(u[j]);
+        if (kOnce && mine > kRing) {
+          // (add() has used u: its place is free)
+          for (int j = 0; j < U; ++j)
+            if (k + kRing + j < mine) {
+              copy_whole(k + kRing + j);
+              if (!whole(k + kRing + j)) at[place(k + kRing + j)] = edge(tid + (k + kRing + j) * NT);
+            }
+          copy_commit();
+        }
       }
       if (OP != kDistill) copy_wait(0);
       if (k < mine) {
         uint4 u[U];
 #pragma unroll
         for (int j = 0; j < U; ++j)
-          u[j] = k + j < mine ? at[(k + j) * NT] : make_uint4(none, none, none, none);
-        take(u);
+          u[j] = k + j < mine ? at[place(k + j)] : make_uint4(none, none, none, none);
+        if (k == 0) {
+#pragma unroll
+          for (int j = 0; j < U; ++j) largest(u[j]);
+          relative_to_m();
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) add(u[j]);
       }
-      rest = warp_join({m, (s0.x + s0.y) + (s1.x + s1.y)}, a.c);
+      if (!(sum() < INFINITY)) {
+        for (k = 0; k < mine; ++k) largest(piece(k));
+        relative_to_m();
+        s0 = s1 = make_float2(0.f, 0.f);
+        for (k = 0; k < mine; ++k) add(piece(k));
+      }
+      rest = warp_join({m, sum()}, a.c);
     }
     double qz = 0.0;
     if (!owner) {
@@ -496,26 +547,47 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       tell(&s_qz[rank], qz);
     }
     told();
+    if (OP == kLogp && C == 1 && warp != 0) {
+      // (a far row needs them all once more)
+      bool far = false;
+      for (int i = 0; i < NW; ++i) far = far || is_far(s_rest[i].m);
+      if (!far) return;
+    }
     rest = {-INFINITY, 0.f};
     if (lane < C * NW) rest = s_rest[lane];
     if (C * NW > 32 && lane + 32 < C * NW) rest = join(rest, s_rest[lane + 32], a.c);
     rest = warp_join(rest, a.c);
     if (is_far(rest.m)) {
-      const Form f = form_of(rest.m, a.c);
-      float s = 0.f;
+      // the row's maximum, which is not that of the first pieces, and the sum
+      // in its form: two exchanges more
+      auto exchange = [&](float v, float* slots) {
+        if (owner) tell(&slots[rank * NW + warp], v);
+        told();
+      };
+      float v = -INFINITY;
       for (int k = 0; k < mine; ++k) {
         float2 x[EI / 2];
-        unpack(at[k * NT], x, (const TI*)nullptr);
+        unpack(piece(k), x, (const TI*)nullptr);
+#pragma unroll
+        for (int i = 0; i < EI / 2; ++i) v = tc::fmax3(v, x[i].x, x[i].y);
+      }
+      exchange(warp_max_redux(v), s_again);
+      v = -INFINITY;
+      for (int i = lane; i < C * NW; i += 32) v = fmaxf(v, s_again[i]);
+      rest.m = warp_max_redux(v);
+      const Form f = form_of(rest.m, a.c);
+      v = 0.f;
+      for (int k = 0; k < mine; ++k) {
+        float2 x[EI / 2];
+        unpack(piece(k), x, (const TI*)nullptr);
 #pragma unroll
         for (int i = 0; i < EI / 2; ++i)
-          s += tc::fast_exp2(fmaf(x[i].x, f.c, -f.b)) + tc::fast_exp2(fmaf(x[i].y, f.c, -f.b));
+          v += tc::fast_exp2(fmaf(x[i].x, f.c, -f.b)) + tc::fast_exp2(fmaf(x[i].y, f.c, -f.b));
       }
-      s = warp_sum(s);
-      if (owner) tell(&s_again[rank * NW + warp], s);
-      told();
-      s = lane < C * NW ? s_again[lane] : 0.f;
-      if (C * NW > 32 && lane + 32 < C * NW) s += s_again[lane + 32];
-      rest.s = warp_sum(s);
+      exchange(warp_sum(v), s_again + kMaxCluster * NW);
+      v = 0.f;
+      for (int i = lane; i < C * NW; i += 32) v += s_again[kMaxCluster * NW + i];
+      rest.s = warp_sum(v);
     }
     if (OP == kDistill) {
       MaxSum one = {-INFINITY, 0.f};
@@ -698,7 +770,7 @@ __global__ void __launch_bounds__(1024) k_scaled_sum(const float* l, int64_t n, 
 }
 
 template <RowOp OP, typename TI, typename TO>
-__global__ void __launch_bounds__(kThreadsOf<OP>, 3) k_vocab_row(const RowArgs a) {
+__global__ void __launch_bounds__(kThreadsOf<OP>, kCtasPerSM<OP>) k_vocab_row(const RowArgs a) {
   if (OP == kLogpBwd) {
     // it has nothing to exchange: plain CTAs.  Last rows first: they are the
     // ones that the log-probabilities' pass has left in L2
@@ -791,16 +863,20 @@ void allow_shared_memory(const void* kern) {
 }
 
 // How the rows are laid out over CTAs: as few of them per row as hold its
-// 16-byte pieces when three CTAs share an SM, and at most kMaxCluster.
+// 16-byte pieces when three CTAs share an SM, more of them where the rows are
+// too few to occupy the SMs (down to 16 KB each), and at most kMaxCluster.
+// `once`: the pieces pass through a ring and need not fit.
 struct Split {
   int cluster, share;  // CTAs per row; pieces per CTA
 };
-Split split_of(int64_t rows, int64_t vocab, int prec, int64_t lists) {
+Split split_of(int64_t rows, int64_t vocab, int prec, int64_t lists, bool once) {
   // the pieces that a row touches wherever it starts
   const int64_t size = prec == DOP_BF16 ? 2 : 4, pieces = ceil_div(vocab * size + 16 - size, 16);
-  const int64_t C = std::min<int64_t>(ceil_div(16 * pieces, kCtaBytes - lists), kMaxCluster);
+  const int64_t fit = once ? 1 : ceil_div(16 * pieces, kCtaBytes - lists);
+  const int64_t fill = std::min(ceil_div(3 * sm_count(), std::max<int64_t>(rows, 1)), ceil_div(pieces, 1024));
+  const int64_t C = std::min<int64_t>(std::max(fit, fill), kMaxCluster);
   const int64_t share = ceil_div(pieces, C);
-  if (16 * share > kStageBytesMost)
+  if (!once && 16 * share > kStageBytesMost)
     throw Error(DOP_E_UNSUPPORTED, "vocab (" + std::to_string(vocab) + ") is above " +
                                        std::to_string((C * kStageBytesMost - 16) / size + 1));
   if (rows * C >= INT32_MAX) throw Error(DOP_E_UNSUPPORTED, "too many rows for this vocab");
@@ -836,10 +912,10 @@ template <RowOp OP>
 void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t s) {
   if (rows == 0) return;
   const int64_t lists = OP == kDistill ? list_bytes(a.K) : 0;
-  const Split sp = split_of(rows, a.V, prec, lists);
+  const Split sp = split_of(rows, a.V, prec, lists, OP == kLogp);
   a.cluster = sp.cluster;
   a.share = sp.share;
-  a.stage_bytes = 16 * sp.share;
+  a.stage_bytes = 16 * (OP == kLogp ? std::min(sp.share, kRing * kOwnersOf<OP>) : sp.share);
   a.rows = rows;
   const int64_t ctas = rows * a.cluster + (a.sum_of ? 1 : 0);
   by_types(prec, grad_prec, a.dz != nullptr, [&](auto ti, auto to) {
@@ -855,7 +931,7 @@ void check_rows(int64_t rows, int64_t vocab, int prec, const void* z, int64_t ld
   DOP_REQUIRE(rows >= 0 && rows <= INT32_MAX, "rows must lie in [0, 2^31)");
   DOP_REQUIRE(vocab >= 1 && vocab <= INT32_MAX, "vocab must lie in [1, 2^31)");
   DOP_REQUIRE(prec == DOP_F32 || prec == DOP_BF16, "unknown precision");
-  split_of(rows, vocab, prec, 0);
+  split_of(rows, vocab, prec, 0, false);
   DOP_REQUIRE(ld >= vocab, "the logits' row stride is smaller than vocab");
   DOP_REQUIRE(z || rows == 0, "null logits");
   DOP_REQUIRE((uintptr_t)z % elem_bytes(prec) == 0, "misaligned logits");
