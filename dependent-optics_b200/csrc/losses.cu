@@ -31,17 +31,33 @@ int set_last_error(int code, const char* msg);
 
 namespace {
 
-enum RowOp : int { kLogp = 0, kLogpBwd = 1, kPolicy = 2, kDistill = 3 };
+// (kDistillRest: distillation with a class for the entries outside the list)
+enum RowOp : int { kLogp = 0, kLogpBwd = 1, kPolicy = 2, kDistill = 3, kDistillRest = 4 };
+constexpr bool has_list(RowOp op) { return op == kDistill || op == kDistillRest; }
 
-constexpr int kRowThreads = 256;
 constexpr int kMaxTeacherK = 1024;
-constexpr int kMaxCluster = 8;
-constexpr int kOnceThreads = 128, kOnceCtas = 8;
-constexpr int kRing = 8;  // pieces that a thread reading a row once has under way
-// Shared memory: of a CTA when three are to fit an SM (of its 228 KB, less the
-// static share and what the system takes of each), and of a CTA's pieces at most.
-constexpr int64_t kCtaBytes = 228 * 1024 / 3 - 2560, kStageBytesMost = 200 * 1024;
 constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
+constexpr int kMaxCluster = 8;
+// CTAs by the pieces that they keep.  Narrow: 128 threads with up to 16 pieces
+// each in shared memory (32 KB of a row), six CTAs an SM; pieces that are read
+// once pass through 8 or 16 places.  Held: 256 threads, up to 18 pieces (72
+// KB), three CTAs an SM.  Wide: 16 pieces more per thread in tensor memory,
+// 128 KB, three CTAs an SM.  Alone: at most 40 and 64 pieces (416 KB), one CTA
+// an SM.
+//
+// A CTA that holds tensor memory waits for the others of its cluster, so the
+// CTAs that may share an SM must never ask for more than its 512 columns: 64
+// KB of shared memory go with every 128 columns (three at most), and one that
+// takes them all takes the shared memory that another would need.
+enum Shape : int { kNarrow, kHeld, kWide, kAlone };
+constexpr int owners_of(Shape s) { return s == kNarrow ? 128 : 256; }
+// Columns of tensor memory.  A constant in the instruction, and kernels
+// without it for the shapes that take none: CTAs of a kernel that names
+// tensor memory start about half a microsecond apart on an SM.
+constexpr int columns_of(Shape s) { return s == kWide ? 128 : s == kAlone ? 512 : 0; }
+constexpr int kKept = 16, kHeldMost = 18, kPassing = 8, kRingMost = 40, kMovedMost = 64;
+constexpr int64_t kAloneBytes = 200 * 1024;
+constexpr int kPairThreads = 256;
 
 struct RowArgs {
   const void* z;
@@ -58,8 +74,10 @@ struct RowArgs {
   int64_t sum_n;        // taken with the adjoint
   float* loss;
   int cluster;      // CTAs per row
-  int share;        // 16-byte pieces of a row a CTA has
-  int stage_bytes;  // of shared memory for a CTA's pieces
+  int share;         // 16-byte pieces of a row a CTA has
+  int ring;          // places for pieces per thread in shared memory
+  int stage_bytes;   // all of them
+  int bit_words;     // of the list's bits
   double scale;  // of the loss and the adjoint
   float* logp;
   float* logp_lo;  // null, or what logp's rounding to fp32 left out
@@ -138,16 +156,21 @@ __device__ double block_sum_d(double v, double* red) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   double t = 0.0;
-  for (int w = 0; w < kRowThreads / 32; ++w) t += red[w];
+  for (int w = 0; w < kPairThreads / 32; ++w) t += red[w];
   return t;
 }
 
-// ---- a row in shared memory
+// ---- a row on the SM
 // A row is cut into 16-byte pieces at 16-byte borders of its address, so a
 // row may start and end inside a piece; the cluster's CTAs hold consecutive
-// runs of pieces, one CTA the whole row when it fits.  A thread copies pieces
-// tid, tid + 256, ... and is the one that reads them back for the maximum and
-// sum, so that pass needs no barrier.  What a piece holds beyond the row is -inf.
+// runs of pieces, one CTA the whole row when it fits.  Thread t owns pieces t,
+// t + NT, ... of its CTA: it copies them, reads them for the maximum and sum
+// and again for the adjoint, so that neither needs a barrier.  They come
+// through a ring in shared memory, in groups of U pieces a thread; a group
+// whose place in the ring is wanted for a later one moves to the thread's own
+// lane of tensor memory, whose 256 KB double what an SM can hold of the rows
+// under way.  What is kept is the bf16 logits, or of fp32 logits the powers
+// of two themselves.  What a piece holds beyond the row is -inf.
 __device__ __forceinline__ void copy_piece(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -164,6 +187,10 @@ __device__ __forceinline__ void copy_wait(int n) {
     case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
     default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
   }
+}
+template <int N>
+__device__ __forceinline__ void copy_wait_for() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ float2 bf16x2(uint32_t u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
@@ -193,10 +220,37 @@ __device__ __forceinline__ void store_n(bf16* p, const float (&v)[8]) {
                                             tc::pack_bf16(v[4], v[5]), tc::pack_bf16(v[6], v[7]));
 }
 
-// Bits of the filter that finds out whether a list may name an entry twice.
-constexpr int kFilterBits = 32768;
+// The same where the address is only a multiple of the element: `off` is its
+// remainder by the size of the N elements.
+__device__ __forceinline__ void store_off(float* p, const float (&v)[4], int off) {
+  if (off == 8) {
+    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    *reinterpret_cast<float2*>(p + 2) = make_float2(v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = v[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_off(bf16* p, const float (&v)[N], int off) {
+  if (off % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+      *reinterpret_cast<uint32_t*>(p + i) = tc::pack_bf16(v[i], v[i + 1]);
+  } else {
+    st(p, v[0]);
+#pragma unroll
+    for (int i = 1; i + 1 < N; i += 2)
+      *reinterpret_cast<uint32_t*>(p + i) = tc::pack_bf16(v[i], v[i + 1]);
+    st(p + N - 1, v[N - 1]);
+  }
+}
+
 // A list's arrays start at 16-byte borders.
 __host__ __device__ constexpr int list_stride(int K) { return (K + 3) & ~3; }
+// Bits of the filter that finds out whether a list may name an entry twice
+// (where it need not say which entries are listed).
+constexpr int kFilterBits = 8192;
 
 // ln(s), to about 2^-24 of it or of 1: the exponent apart (0, subnormal, inf
 // and NaN as log has them).
@@ -206,19 +260,69 @@ __device__ __forceinline__ double ln(float s) {
   return (double)e * kLn2 + (double)logf(__int_as_float(__float_as_int(s) - (e << 23)));
 }
 
-// A cluster of a.cluster CTAs per row: 256 threads own the pieces, and
-// distillation has a warp more for the teacher's list.
-template <RowOp OP>
-constexpr int kOwnersOf = OP == kLogp ? kOnceThreads : kRowThreads;
-template <RowOp OP>
-constexpr int kThreadsOf = kOwnersOf<OP> + (OP == kDistill ? 32 : 0);
-template <RowOp OP>
-constexpr int kCtasPerSM = OP == kLogp ? kOnceCtas : 3;
+// Pieces that are in part outside the row, and element by element: out of
+// line, since the CTAs of an SM share its instruction cache.
+template <typename T>
+__device__ __noinline__ uint4 part_of_row(const T* z, int e, int V) {  // piece at element e
+  constexpr int N = 16 / (int)sizeof(T);
+  T v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = e + i >= 0 && e + i < V ? z[e + i] : (T)-INFINITY;
+  uint4 u;
+  memcpy(&u, v, 16);
+  return u;
+}
+template <typename T>
+__device__ __noinline__ void store_elements(T* dz, int e, int V, int n, float4 a, float4 b) {
+  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n && e + i >= 0 && e + i < V) st(&dz[e + i], v[i]);
+}
 
-template <RowOp OP, typename TI, typename TO>
+template <int N>
+__device__ __forceinline__ void alloc_columns(uint32_t slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "n"(N));
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+// Two pieces to eight columns of the thread's lane, and back.
+__device__ __forceinline__ void tmem_put(uint32_t at, const uint4 (&u)[2]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at),
+               "r"(u[0].x), "r"(u[0].y), "r"(u[0].z), "r"(u[0].w), "r"(u[1].x), "r"(u[1].y),
+               "r"(u[1].z), "r"(u[1].w)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_get(uint32_t at, uint4 (&u)[2]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(u[0].x), "=r"(u[0].y), "=r"(u[0].z), "=r"(u[0].w), "=r"(u[1].x), "=r"(u[1].y),
+        "=r"(u[1].z), "=r"(u[1].w)
+      : "r"(at)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void free_columns(uint32_t at) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "n"(N));
+}
+
+// A row by a cluster of a.cluster CTAs, of which NT threads own the pieces;
+// distillation has a warp more for the teacher's list.
+template <RowOp OP, Shape S>
+constexpr int kThreadsOf = owners_of(S) + (has_list(OP) ? 32 : 0);
+template <RowOp OP, Shape S>
+constexpr int kCtasPerSM = S == kAlone ? 1 : S != kNarrow ? 3 : OP == kLogp ? 8 : 6;
+
+template <RowOp OP, typename TI, typename TO, Shape S>
 __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, const int rank) {
   constexpr int EI = 16 / (int)sizeof(TI);
-  constexpr int NT = kOwnersOf<OP>, NW = NT / 32, U = OP == kLogp ? 2 : 4;
+  constexpr int NT = owners_of(S), NW = NT / 32, THREADS = kThreadsOf<OP, S>;
+  constexpr bool kOnce = OP == kLogp || OP == kLogpBwd;  // the pieces are read once
+  constexpr bool kList = has_list(OP), tail = OP == kDistillRest;
+  constexpr bool kKeepPower = sizeof(TI) == 4 && !kOnce;
+  constexpr bool kTmem = !kOnce && columns_of(S) > 0;
+  constexpr bool kFits = !kOnce && !kTmem;  // every piece has a place of its own
+  constexpr int U = kFits ? 4 : 2;
   extern __shared__ __align__(16) uint8_t dyn[];
   // of every warp of the cluster
   __shared__ MaxSum s_rest[kMaxCluster * NW];
@@ -227,11 +331,11 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
   __shared__ __align__(16) float4 s_listed[kMaxCluster];
   __shared__ double s_qz[kMaxCluster];
   __shared__ double s_q[3];
-  __shared__ int s_twice;
+  __shared__ uint32_t s_tmem;
   const int C = a.cluster, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool owner = OP != kDistill || tid < NT;  // of pieces
+  const bool owner = !kList || tid < NT;  // of pieces
   const float w = a.weight ? a.weight[row] : 1.f;
-  const int64_t token64 = OP == kDistill ? -1 : a.tokens[row];
+  const int64_t token64 = kList ? -1 : a.tokens[row];
   const float dlogp = OP == kLogpBwd ? a.dlogp[row] : 0.f;
   const float lse_in = OP == kLogpBwd ? a.lse[row] : 0.f;
   const float adv = OP == kPolicy ? a.advantage[row] : 0.f;
@@ -240,7 +344,7 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
 
   int32_t my_idx = -1;
   float my_top = 0.f;
-  if (OP == kDistill && tid < NT && tid < a.K) {
+  if (kList && owner && tid < a.K) {
     my_idx = a.top_index[row * a.K + tid];
     my_top = a.top_logit[row * a.K + tid];
   }
@@ -252,147 +356,170 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
   const int ph = (int)((uintptr_t)z & 15) / (int)sizeof(TI);
   const int pieces = (ph + V + EI - 1) / EI;
   const int p0 = min(pieces, rank * a.share), np = min(pieces, p0 + a.share) - p0;
-  const int e_org = p0 * EI - ph;  // the row's element at image element 0
+  const int e_org = p0 * EI - ph;  // the row's element where its pieces start
   const int e_lo = max(0, e_org), e_hi = max(e_lo, min(V, e_org + np * EI));
   // pieces that lie in the row altogether: [f0, f1)
   const int f0 = e_org < 0 ? 1 : 0, f1 = e_org + np * EI > V ? np - 1 : np;
 
-  if (w == 0.f || row < a.in_lo || row >= a.in_hi || (OP != kDistill && (token64 < 0 || token64 >= V)) ||
+  if (w == 0.f || row < a.in_lo || row >= a.in_hi || (!kList && (token64 < 0 || token64 >= V)) ||
       (OP == kLogpBwd && dlogp == 0.f)) {
     if (dz) {
       constexpr int EO = 16 / (int)sizeof(TO);
       const int dph = (int)((uintptr_t)dz & 15) / (int)sizeof(TO);
       const int u0 = (dph + e_lo + EO - 1) / EO, u1 = (dph + e_hi) / EO;  // 16-byte units
       const int ahead = u0 < u1 ? u0 * EO - dph : e_hi, behind = u0 < u1 ? u1 * EO - dph : e_hi;
-      for (int u = u0 + tid; u < u1; u += kThreadsOf<OP>)
+      for (int u = u0 + tid; u < u1; u += THREADS)
         *reinterpret_cast<uint4*>(dz + (u * EO - dph)) = make_uint4(0u, 0u, 0u, 0u);
       if (e_lo + tid < ahead) st(&dz[e_lo + tid], 0.f);
       if (behind + tid < e_hi) st(&dz[behind + tid], 0.f);
     }
     if (tid == 0 && rank == 0) {
-      if (OP != kLogpBwd && OP != kDistill && a.logp) a.logp[row] = 0.f;
+      if (OP != kLogpBwd && !kList && a.logp) a.logp[row] = 0.f;
       if (OP == kLogp && a.lse) a.lse[row] = 0.f;
       if (OP == kLogp && a.logp_lo) a.logp_lo[row] = 0.f;
-      if (OP == kPolicy || OP == kDistill) a.row_loss[row] = 0.f;
+      if (OP == kPolicy || kList) a.row_loss[row] = 0.f;
     }
     return;
   }
-  constexpr bool stats = OP != kLogpBwd;  // it has lse
   // every CTA of the cluster has started once this barrier is through: its
   // shared memory may be written to
-  if (stats && C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (OP != kLogpBwd && C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
-  // ---- copy this CTA's pieces; a thread owns pieces tid + NT k, and the
-  // first `mine` of them are the row's
-  // (the log-probability reads its pieces once, in a ring of kRing of them)
-  constexpr bool kOnce = OP == kLogp;
-  TI* image = (TI*)dyn;
-  uint4* at = (uint4*)dyn + tid;  // piece k: at[k NT], in the ring at[(k % kRing) NT]
-  auto place = [&](int k) { return kOnce ? (k % kRing) * NT : k * NT; };
-  const int mine = owner && tid < np ? (np - tid + NT - 1) / NT : 0;
-  // the first and the last piece of the row may be in part outside it
-  auto edge = [&](int i) {
-    TI v[EI];
-#pragma unroll
-    for (int k = 0; k < EI; ++k) {
-      const int e = e_org + i * EI + k;
-      v[k] = e >= 0 && e < V ? z[e] : (TI)-INFINITY;
-    }
-    uint4 u;
-    memcpy(&u, v, 16);
-    return u;
-  };
+  // ---- copy the first groups of pieces
+  // groups of the CTA, places for them in the ring, and those that tensor
+  // memory takes over (all the same for every thread)
+  const int groups = (np + NT * U - 1) / (NT * U), ring = kFits ? groups : a.ring / U;
+  const int moved = dz && kTmem ? max(0, groups - ring) : 0;
+  const int mine = owner && tid < np ? (np - tid + NT - 1) / NT : 0;  // pieces of this thread
+  uint4* at = (uint4*)dyn + tid;  // piece j of place r: at[(r U + j) NT]
+  auto edge = [&](int i) { return part_of_row(z, e_org + i * EI, V); };
   const uint4* src = (const uint4*)(z + e_org) + tid;
   const uint32_t dst = tc::smem_u32(at);
   auto whole = [&](int k) { return tid + k * NT >= f0 && tid + k * NT < f1; };
-  auto copy_whole = [&](int k) {
-    if (whole(k)) copy_piece(dst + place(k) * 16, src + k * NT);
-  };
-  if (owner) {
-    const int n = kOnce ? min(mine, kRing) : mine;
-    int k = 0;
-    for (; k + U <= n; k += U) {
-      if (tid + k * NT >= f0 && tid + (k + U - 1) * NT < f1) {
+  auto copy_group = [&](int g, int r) {  // group g to place r
+    if (tid + g * U * NT >= f0 && tid + (g * U + U - 1) * NT < f1) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) copy_piece(dst + place(k + j) * 16, src + (k + j) * NT);
-      } else {
-        for (int j = 0; j < U; ++j) copy_whole(k + j);
-      }
-      copy_commit();
+      for (int j = 0; j < U; ++j) copy_piece(dst + (r * U + j) * (NT * 16), src + (g * U + j) * NT);
+    } else {
+      for (int j = 0; j < U; ++j)
+        if (whole(g * U + j)) copy_piece(dst + (r * U + j) * (NT * 16), src + (g * U + j) * NT);
     }
-    for (; k < n; ++k) copy_whole(k);
     copy_commit();
-    // the two that a row may share with what lies beside it, while the copies run
-    if (f0 == 1 && tid == 0 && n > 0) at[0] = edge(0);
-    if (f1 < np && f1 >= f0 && tid == f1 % NT && f1 / NT < n) at[place(f1 / NT)] = edge(f1);
-  }
-  // piece k once more, after its copy (a ring may have given it up)
-  auto piece = [&](int k) {
-    const int i = tid + k * NT;
-    return !kOnce ? at[k * NT] : i >= f0 && i < f1 ? src[k * NT] : edge(i);
   };
-  const float za = OP == kDistill || OP == kLogpBwd ? 0.f : ld(&z[token]);
+  // the pieces of a group that are in part outside the row: at most the
+  // row's first and its last
+  auto copy_edges = [&](int g, int r) {
+#pragma unroll 1
+    for (int j = 0; j < U; ++j)
+      if (g * U + j < mine && !whole(g * U + j)) at[(r * U + j) * NT] = edge(tid + (g * U + j) * NT);
+  };
+  const int g_head = f0 == 1 ? 0 : -1, g_tail = f1 < np ? f1 / (NT * U) : -1;
+  const int first = min(groups, ring);
+  if (owner) {
+    for (int g = 0; g < first; ++g) copy_group(g, g);
+    if (g_head >= 0 && g_head < first && tid == 0) copy_edges(g_head, g_head);
+    if (g_tail >= 0 && g_tail < first && tid == f1 % NT) copy_edges(g_tail, g_tail);
+  }
+  if constexpr (kTmem)
+    if (warp == 0) {
+      __syncwarp();
+      alloc_columns<columns_of(S)>(tc::smem_u32(&s_tmem));
+    }
+  const float za = OP == kLogp || OP == kPolicy ? ld(&z[token]) : 0.f;
 
-  // ---- the teacher's list leaves the image.  While the copies run, the
-  // owners put the list into shared memory and find out whether an entry may
-  // be named twice (two entries on one bit of a filter); the warp that owns
-  // no pieces works out q while the others take the maximum and sum.
-  const int K4 = OP == kDistill ? list_stride(a.K) : 0;
+  // ---- the teacher's list, by the warp that owns no pieces
+  const int K4 = kList ? list_stride(a.K) : 0;
   int32_t* t_idx = (int32_t*)(dyn + a.stage_bytes);
   float* t_q = (float*)t_idx + K4;  // the teacher's logit, then q
   float* t_z = t_q + K4;            // the student's logit, of this CTA's entries
   float* t_g = t_z + K4;            // this CTA's first ones: sum of q of the entry; else -1
-  if (OP == kDistill) {
-    uint32_t* filter = (uint32_t*)(t_g + K4);
+  // with a class for the rest, one bit per element of this CTA: whether it is
+  // listed; else a filter
+  uint32_t* bits = (uint32_t*)(t_g + K4);
+  if (kList) {
+    // its owners bring the list while their copies run, and go on; the warp
+    // without pieces takes it from there
     if (owner) {
-      for (int i = tid; i < kFilterBits / 128; i += NT) ((uint4*)filter)[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (tid == 0) s_twice = 0;
-      asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
+#pragma unroll 1
       for (int k = tid; k < a.K; k += NT) {
         const int32_t i = k < NT ? my_idx : a.top_index[row * a.K + k];
         const float y = k < NT ? my_top : a.top_logit[row * a.K + k];
-        const bool in = i >= 0 && i < V;
+        const bool in = i >= 0 && i < V, here = i >= e_lo && i < e_hi;
         t_idx[k] = in ? i : -1;
         t_q[k] = in ? y : -INFINITY;
-        if (in) {
-          const uint32_t h = (uint32_t)i % kFilterBits, bit = 1u << (h & 31);
-          if (atomicOr(&filter[h >> 5], bit) & bit) s_twice = 1;
-        }
+        t_z[k] = here ? ld(&z[i]) : 0.f;
+        t_g[k] = here ? 0.f : -1.f;
       }
-    }
-    copy_wait(0);
-    __syncthreads();
-    for (int k = tid; k < a.K; k += kThreadsOf<OP>) {
-      const int i = t_idx[k];
-      const bool here = i >= e_lo && i < e_hi;
-      t_z[k] = here ? ld(&image[i - e_org]) : 0.f;
-      t_g[k] = here ? 0.f : -1.f;
-      if (!s_twice && here) image[i - e_org] = (TI)-INFINITY;
-    }
-    __syncthreads();
-    if (s_twice) {
-      for (int k = tid; k < a.K; k += kThreadsOf<OP>)
-        if (t_g[k] == 0.f) image[t_idx[k] - e_org] = (TI)-INFINITY;
-      __syncthreads();
+      asm volatile("bar.arrive 1, %0;" ::"n"(THREADS) : "memory");
+    } else {
+      asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
     }
   }
+  auto set_bits = [&] {
+#pragma unroll 1
+    for (int i = lane; i < a.bit_words; i += 32) bits[i] = 0u;
+    __syncwarp();
+    bool twice = false;
+#pragma unroll 1
+    for (int k = lane; k < a.K; k += 32)
+      if (!(t_g[k] < 0.f)) {
+        const int i = t_idx[k];
+        const uint32_t h = tail ? (uint32_t)(i - e_org) : (uint32_t)i % kFilterBits, bit = 1u << (h & 31);
+        if (atomicOr(&bits[h >> 5], bit) & bit) twice = true;
+      }
+    return (bool)__any_sync(0xffffffffu, twice);
+  };
+  // first ones of a list that may name an entry twice get the sum of q, the
+  // others -1
+  auto count_once = [&] {
+#pragma unroll 1
+    for (int k = lane; k < a.K; k += 32) {
+      const int i = t_idx[k];
+      if (t_g[k] < 0.f) continue;
+      double sum = 0.0;
+      bool before = false;
+#pragma unroll 1
+      for (int j = 0; j < a.K; ++j)
+        if (t_idx[j] == i) {
+          if (j < k) before = true;
+          sum += (double)t_q[j];
+        }
+      t_g[k] = before ? -1.f : (float)sum;
+    }
+    __syncwarp();
+  };
+  bool twice = false;
+  if (tail && !owner) twice = set_bits();
+  if (tail || kTmem) {
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+  }
+  // this thread's lane of tensor memory; the second four warps have the
+  // columns behind those of the first four
+  const uint32_t lane_tmem = kTmem ? s_tmem + ((uint32_t)(warp & 3) << 21) +
+                                         (warp >= 4 ? (uint32_t)columns_of(S) / 2 : 0u)
+                                   : 0u;
   // q of the list, its sums, and which entries are a vocabulary entry's first
   auto make_q = [&] {
     MaxSum t = {-INFINITY, 0.f};
     double tl = 0.0;
-    if (a.teacher_lse) {
+    if (tail) {
       tl = (double)a.teacher_lse[row];
     } else {
+#pragma unroll 1
       for (int k = lane; k < a.K; k += 32) t.m = fmaxf(t.m, t_q[k]);
       t.m = warp_max_redux(t.m);
       const Form f = form_of(t.m, a.c);
+#pragma unroll 1
       for (int k = lane; k < a.K; k += 32) t.s += tc::fast_exp2(fmaf(t_q[k], f.c, -f.b));
       tl = ln(warp_sum(t.s));
     }
     double qs = 0.0, ql = 0.0;
+#pragma unroll 1
     for (int k = lane; k < a.K; k += 32) {
       const float y = t_q[k];
-      const double lq = (a.teacher_lse ? (double)y * a.inv_tau : above(y, t.m, a.c, a.inv_tau)) - tl;
+      const double lq = (tail ? (double)y * a.inv_tau : above(y, t.m, a.c, a.inv_tau)) - tl;
       const float hi = (float)lq;  // q to fp32's last digits: lq rounded, the rest applied
       const float q = y == -INFINITY ? 0.f : expf(hi) * (1.f + (float)(lq - (double)hi));
       t_q[k] = q;
@@ -403,30 +530,99 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     qs = warp_sum_d(qs);
     ql = warp_sum_d(ql);
     __syncwarp();
-    if (s_twice)
-      for (int k = lane; k < a.K; k += 32) {
-        const int i = t_idx[k];
-        if (t_g[k] < 0.f) continue;
-        double sum = 0.0;
-        bool first = true;
-        for (int j = 0; j < a.K; ++j)
-          if (t_idx[j] == i) {
-            if (j < k) first = false;
-            sum += (double)t_q[j];
-          }
-        t_g[k] = first ? (float)sum : -1.f;
-      }
-    __syncwarp();
     if (lane == 0) {
       s_q[0] = qs;
       s_q[1] = ql;
+      // (asked of the argument: with a 0 that the compiler knows, its code for
+      // all that follows takes 912 us instead of 839 for 32768 rows of 32000 bf16)
       s_q[2] = a.teacher_lse ? fmax(0.0, 1.0 - qs) : 0.0;
     }
   };
 
-  // ---- maximum and sum
-  MaxSum rest = {-INFINITY, 0.f}, listed = {-INFINITY, 0.f};
-  float count = 0.f;
+  // ---- groups of pieces
+  const uint32_t none = minus_inf_word((const TI*)nullptr);
+  auto in_ring = [&](int g, int r, uint4 (&u)[U]) {
+    if ((g + 1) * U * NT <= np) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) u[j] = at[(r * U + j) * NT];
+    } else {
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        u[j] = g * U + j < mine ? at[(r * U + j) * NT] : make_uint4(none, none, none, none);
+    }
+  };
+  auto anew = [&](int g, uint4 (&u)[U]) {  // from the logits
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = g * U + j;
+      u[j] = k >= mine ? make_uint4(none, none, none, none) : whole(k) ? src[k * NT] : edge(tid + k * NT);
+    }
+  };
+  // listed elements count as -inf where the rest is a class of its own
+  auto without_listed = [&](int g, uint4 (&u)[U]) {
+    if constexpr (tail) {
+      uint32_t m[U];
+  #pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int k = g * U + j, e = (tid + k * NT) * EI;
+        m[j] = k < mine ? bits[e >> 5] >> (e & 31) & ((1u << EI) - 1) : 0u;
+      }
+  #pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (m[j]) {
+          uint32_t* word = &u[j].x;
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t half = EI == 8 ? (m[j] >> (2 * i) & 1 ? 0xffffu : 0u) | (m[j] >> (2 * i + 1) & 1 ? 0xffff0000u : 0u)
+                                          : (m[j] >> i & 1 ? 0xffffffffu : 0u);
+            word[i] = (word[i] & ~half) | (none & half);
+          }
+        }
+    }
+  };
+  // a group whose maximum and sum have been taken
+  auto keep = [&](int g, int r, const uint4 (&u)[U]) {
+    if (kOnce || !dz) return;
+    if (g < moved) {
+      if constexpr (kTmem) {
+        __syncwarp();
+        tmem_put(lane_tmem + (uint32_t)(g * 4 * U), u);
+      }
+    } else if (kKeepPower) {
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (!kFits || g * U + j < mine) at[(r * U + j) * NT] = u[j];
+    }
+  };
+  auto kept = [&](int g, int r, uint4 (&u)[U]) {
+    if constexpr (kTmem)
+      if (g < moved) {
+        __syncwarp();
+        tmem_get(lane_tmem + (uint32_t)(g * 4 * U), u);
+        return;
+      }
+#pragma unroll
+    for (int j = 0; j < U; ++j) u[j] = at[(r * U + j) * NT];
+  };
+  // wait for group g's copies: `first` groups were under way at the start, and
+  // one more is whenever one has been used
+  // (where all are under way at the start, for all: it is less to execute)
+  auto wait_group = [&](int g) {
+    if (groups > ring && OP == kLogp) copy_wait_for<kPassing / U - 1>();
+    else if (!kFits && groups > ring) copy_wait_for<kKept / U - 1>();
+    else if (g == 0) copy_wait_for<0>();
+  };
+  auto refill = [&](int g, int r) {  // place r, which held group g
+    if (kFits || groups <= ring) return;
+    const int next = g + ring;
+    if (next < groups) {
+      copy_group(next, r);
+      if (next == g_tail && tid == f1 % NT) copy_edges(next, r);
+    } else {
+      copy_commit();
+    }
+  };
+
   // v to slot `to` of every CTA of the cluster (lane r: of CTA r)
   auto tell = [&](auto* to, auto v) {
     if (C == 1) {
@@ -444,99 +640,102 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     if (C > 1) tc::cluster_sync();
     else __syncthreads();
   };
-  if constexpr (stats) {
-    const uint32_t none = minus_inf_word((const TI*)nullptr);
-    if (owner) {
-      // the sum is taken relative to the largest of the first pieces; should
-      // a later element pass that by 2^127, the sum says so and is taken
-      // again relative to the maximum of all
-      float m = -INFINITY;
-      float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f), nb = s0;
-      const float2 c2 = make_float2(a.c, a.c);
-      auto largest = [&](uint4 u) {
+
+  // ---- maximum and sum
+  MaxSum rest = {-INFINITY, 0.f}, listed = {-INFINITY, 0.f}, all = {-INFINITY, 0.f};
+  float count = 0.f;
+  float my_base = 0.f;  // the b of this thread's powers
+  if constexpr (OP != kLogpBwd) {
+    float m = -INFINITY;
+    float2 s0 = make_float2(0.f, 0.f), s1 = s0, nb = s0, c2 = make_float2(a.c, a.c);
+    auto largest = [&](const uint4 (&u)[U]) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
         float2 x[EI / 2];
-        unpack(u, x, (const TI*)nullptr);
+        unpack(u[j], x, (const TI*)nullptr);
 #pragma unroll
         for (int i = 0; i < EI / 2; ++i) m = tc::fmax3(m, x[i].x, x[i].y);
-      };
-      auto add = [&](uint4 u) {
+      }
+    };
+    auto add = [&](uint4 (&u)[U]) {  // fp32 logits become their powers
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
         float2 x[EI / 2];
-        unpack(u, x, (const TI*)nullptr);
+        unpack(u[j], x, (const TI*)nullptr);
 #pragma unroll
         for (int i = 0; i < EI / 2; ++i) {
           const float2 t = tc::ffma2(x[i], c2, nb);
           const float2 e = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
           if (i & 1) s1 = tc::fadd2(s1, e);
           else s0 = tc::fadd2(s0, e);
+          x[i] = e;
         }
-      };
-      auto relative_to_m = [&] { nb.x = nb.y = -base_of(m, a.c); };
-      auto sum = [&] { return (s0.x + s0.y) + (s1.x + s1.y); };
-      int k = 0;
-      for (; k + U <= mine; k += U) {
-        // group g of the copies ends with piece (g + 1) U at the latest; a
-        // ring keeps kRing / U groups under way
-        if (kOnce) copy_wait(mine > kRing ? kRing / U - 1 : max(0, mine / U - 1 - k / U));
-        else if (OP != kDistill) copy_wait(max(0, mine / U - 1 - k / U));
-        uint4 u[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) u[j] = at[place(k + j)];
-        if (k == 0) {
-#pragma unroll
-          for (int j = 0; j < U; ++j) largest(u[j]);
-          relative_to_m();
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) add(u[j]);
-        if (kOnce && mine > kRing) {
-          // (add() has used u: its place is free)
-          for (int j = 0; j < U; ++j)
-            if (k + kRing + j < mine) {
-              copy_whole(k + kRing + j);
-              if (!whole(k + kRing + j)) at[place(k + kRing + j)] = edge(tid + (k + kRing + j) * NT);
-            }
-          copy_commit();
-        }
+        if (kKeepPower)
+          u[j] = make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x),
+                            __float_as_uint(x[1].y));
       }
-      if (OP != kDistill) copy_wait(0);
-      if (k < mine) {
-        uint4 u[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-          u[j] = k + j < mine ? at[place(k + j)] : make_uint4(none, none, none, none);
-        if (k == 0) {
-#pragma unroll
-          for (int j = 0; j < U; ++j) largest(u[j]);
-          relative_to_m();
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) add(u[j]);
-      }
-      if (!(sum() < INFINITY)) {
-        for (k = 0; k < mine; ++k) largest(piece(k));
+    };
+    auto relative_to_m = [&] {
+      my_base = base_of(m, a.c);
+      nb = make_float2(-my_base, -my_base);
+    };
+    auto sum = [&] { return (s0.x + s0.y) + (s1.x + s1.y); };
+    uint4 u[U];
+    if (owner) {
+      // relative to the largest of this thread's first pieces
+      if (groups > 0) {
+        wait_group(0);
+        in_ring(0, 0, u);
+        without_listed(0, u);
+        largest(u);
         relative_to_m();
-        s0 = s1 = make_float2(0.f, 0.f);
-        for (k = 0; k < mine; ++k) add(piece(k));
+      }
+      const int full = np / (NT * U);  // groups of which every thread has all pieces
+      for (int g = 0, r = 0; g < full; ++g) {
+        wait_group(g);
+#pragma unroll
+        for (int j = 0; j < U; ++j) u[j] = at[(r * U + j) * NT];
+        without_listed(g, u);
+        add(u);
+        keep(g, r, u);
+        refill(g, r);
+        if (++r == ring) r = 0;
+      }
+      if (full < groups) {
+        const int r = kFits ? full : full % ring;
+        wait_group(full);
+        in_ring(full, r, u);
+        without_listed(full, u);
+        add(u);
+        keep(full, r, u);
       }
       rest = warp_join({m, sum()}, a.c);
     }
     double qz = 0.0;
     if (!owner) {
       make_q();
+#pragma unroll 1
       for (int k = lane; k < a.K; k += 32) {
         const int i = t_idx[k];
         if (i >= e_lo && i < e_hi && t_q[k] != 0.f) qz += (double)t_q[k] * (double)t_z[k];
-        if (t_g[k] < 0.f) continue;
-        listed.m = fmaxf(listed.m, t_z[k]);
-        count += 1.f;
       }
       qz = warp_sum_d(qz);
-      listed.m = warp_max_redux(listed.m);
-      const Form f = form_of(listed.m, a.c);
-      for (int k = lane; k < a.K; k += 32)
-        if (!(t_g[k] < 0.f)) listed.s += tc::fast_exp2(fmaf(t_z[k], f.c, -f.b));
-      listed.s = warp_sum(listed.s);
-      count = warp_sum(count);
+      if (tail) {  // the listed entries' maximum and sum
+        if (twice) count_once();
+#pragma unroll 1
+        for (int k = lane; k < a.K; k += 32)
+          if (!(t_g[k] < 0.f)) {
+            listed.m = fmaxf(listed.m, t_z[k]);
+            count += 1.f;
+          }
+        listed.m = warp_max_redux(listed.m);
+        const Form f = form_of(listed.m, a.c);
+#pragma unroll 1
+        for (int k = lane; k < a.K; k += 32)
+          if (!(t_g[k] < 0.f)) listed.s += tc::fast_exp2(fmaf(t_z[k], f.c, -f.b));
+        listed.s = warp_sum(listed.s);
+        count = warp_sum(count);
+      }
     }
     // every warp's to every CTA of the cluster, joined there in a fixed order
     if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
@@ -547,49 +746,56 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       tell(&s_qz[rank], qz);
     }
     told();
-    if (OP == kLogp && C == 1 && warp != 0) {
-      // (a far row needs them all once more)
-      bool far = false;
-      for (int i = 0; i < NW; ++i) far = far || is_far(s_rest[i].m);
-      if (!far) return;
+    // A sum relative to first pieces says so when a later element passes them
+    // by 2^127, and one of far elements is not one; then all is taken once
+    // more, relative to the maximum of the row.
+    auto not_one = [&](const MaxSum& v) { return is_far(v.m) || !(v.s < INFINITY); };
+    if (OP == kLogp && C == 1 && warp != 0) {  // (which needs every warp)
+      // (short of overflow, so that their joined sum cannot either)
+      bool once_more = false;
+      for (int i = 0; i < NW; ++i) once_more = once_more || is_far(s_rest[i].m) || !(s_rest[i].s < 0x1p120f);
+      if (!once_more) return;
     }
     rest = {-INFINITY, 0.f};
-    if (lane < C * NW) rest = s_rest[lane];
-    if (C * NW > 32 && lane + 32 < C * NW) rest = join(rest, s_rest[lane + 32], a.c);
+    for (int i = lane; i < C * NW; i += 32) rest = join(rest, s_rest[i], a.c);
     rest = warp_join(rest, a.c);
-    if (is_far(rest.m)) {
-      // the row's maximum, which is not that of the first pieces, and the sum
-      // in its form: two exchanges more
+    if (not_one(rest)) {
       auto exchange = [&](float v, float* slots) {
         if (owner) tell(&slots[rank * NW + warp], v);
         told();
       };
-      float v = -INFINITY;
-      for (int k = 0; k < mine; ++k) {
-        float2 x[EI / 2];
-        unpack(piece(k), x, (const TI*)nullptr);
-#pragma unroll
-        for (int i = 0; i < EI / 2; ++i) v = tc::fmax3(v, x[i].x, x[i].y);
-      }
-      exchange(warp_max_redux(v), s_again);
-      v = -INFINITY;
-      for (int i = lane; i < C * NW; i += 32) v = fmaxf(v, s_again[i]);
-      rest.m = warp_max_redux(v);
+      if (owner)
+#pragma unroll 1
+        for (int g = 0; g < groups; ++g) {
+          anew(g, u);
+          without_listed(g, u);
+          largest(u);
+        }
+      exchange(warp_max_redux(m), s_again);
+      m = -INFINITY;
+      for (int i = lane; i < C * NW; i += 32) m = fmaxf(m, s_again[i]);
+      rest.m = warp_max_redux(m);
       const Form f = form_of(rest.m, a.c);
-      v = 0.f;
-      for (int k = 0; k < mine; ++k) {
-        float2 x[EI / 2];
-        unpack(piece(k), x, (const TI*)nullptr);
-#pragma unroll
-        for (int i = 0; i < EI / 2; ++i)
-          v += tc::fast_exp2(fmaf(x[i].x, f.c, -f.b)) + tc::fast_exp2(fmaf(x[i].y, f.c, -f.b));
-      }
-      exchange(warp_sum(v), s_again + kMaxCluster * NW);
-      v = 0.f;
+      c2 = make_float2(f.c, f.c);
+      nb = make_float2(-f.b, -f.b);
+      my_base = base_of(rest.m, a.c);
+      s0 = s1 = make_float2(0.f, 0.f);
+      if (owner)
+#pragma unroll 1
+        for (int g = 0, r = 0; g < groups; ++g) {
+          anew(g, u);
+          without_listed(g, u);
+          add(u);
+          keep(g, r, u);
+          if (++r == ring) r = 0;
+        }
+      exchange(warp_sum(sum()), s_again + kMaxCluster * NW);
+      float v = 0.f;
       for (int i = lane; i < C * NW; i += 32) v += s_again[kMaxCluster * NW + i];
       rest.s = warp_sum(v);
     }
-    if (OP == kDistill) {
+    if constexpr (kTmem) tc::tmem_st_wait();
+    if (tail) {  // (without a class for the rest nothing is listed apart)
       MaxSum one = {-INFINITY, 0.f};
       count = 0.f;
       if (lane < C) {
@@ -599,6 +805,20 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       listed.m = warp_max_redux(one.m);
       listed.s = warp_sum(one.s * rescale(one.m, listed.m, a.c));
       count = warp_sum(count);
+    }
+    all = kList ? join(rest, listed, a.c) : rest;
+    if (kList && is_far(all.m)) {
+      // the sum of q (z - m) instead, which keeps its digits
+      if (!owner) {
+        qz = 0.0;
+#pragma unroll 1
+        for (int k = lane; k < a.K; k += 32)
+          if (t_idx[k] >= e_lo && t_idx[k] < e_hi && t_q[k] != 0.f)
+            qz += (double)t_q[k] * ((double)t_z[k] - (double)all.m);
+        qz = warp_sum_d(qz);
+        tell(&s_qz[rank], qz);
+      }
+      told();
     }
   }
 
@@ -646,7 +866,6 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     hot = (float)(a.scale * a.inv_tau) * (w * d);
     c_out = -hot / rest.s;
   } else {
-    const MaxSum all = join(rest, listed, a.c);
     f_in = form_of(all.m, a.c);
     // without an entry outside the list there is no class for the rest
     const float q_sum = (float)s_q[0], q_rest = count == (float)V ? 0.f : (float)s_q[2];
@@ -661,93 +880,123 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     if (!owner && rank == 0 && lane == 0) {
       const double qs = s_q[0], ls_all = ln(all.s), ls_rest = ln(rest.s);
       double qz = 0.0;
+#pragma unroll 1
       for (int i = 0; i < C; ++i) qz += s_qz[i];
       // sum of q (z / tau - lse), as above() has it of one z
-      const double x = is_far(all.m) ? (qz - qs * (double)all.m) * a.inv_tau
+      const double x = is_far(all.m) ? qz * a.inv_tau
                                      : (qz * (double)a.c - qs * (double)f_in.b) * kLn2;
       double l = s_q[1] - (x - qs * ls_all);
       if (q_rest > 0.f)  // -log of the student's share outside the list
-        l += (double)q_rest * ((double)logf(q_rest) + (ls_all - above(0.f, all.m, a.c, a.inv_tau)) -
-                               (ls_rest - above(0.f, rest.m, a.c, a.inv_tau)));
+        l += (double)q_rest *
+             ((double)logf(q_rest) + (ls_all - ls_rest) -
+              (above(0.f, all.m, a.c, a.inv_tau) - above(0.f, rest.m, a.c, a.inv_tau)));
       a.row_loss[row] = (float)((double)w * l / (a.inv_tau * a.inv_tau));
     }
+    if (!owner && !tail && dz) {
+      __syncwarp();
+      if (set_bits()) count_once();
+    }
   }
-  if (!dz) return;
+  if (!dz) {
+    if constexpr (kTmem) {
+      tc::tc_fence_before();
+      __syncthreads();
+      if (warp == 0) free_columns<columns_of(S)>(s_tmem);
+    }
+    return;
+  }
 
   // ---- the adjoint
-  if (OP == kLogpBwd) copy_wait(0);
+  // powers that were kept are relative to this thread's own base
+  if (kKeepPower && !is_far(rest.m)) c_out *= tc::fast_exp2(my_base - f.b);
   const float2 c2 = make_float2(f.c, f.c), nb = make_float2(-f.b, -f.b);
   const float2 g2 = make_float2(c_out, c_out);
-  auto values = [&](const float2 (&x)[EI / 2], float (&v)[EI], int e) {  // v[0] is element e's
+  const int off = (int)((uintptr_t)(dz + e_org) % (EI * sizeof(TO)));  // of every piece's place in dz
+  auto values = [&](uint4 u, int e, float (&v)[EI]) {  // v[0] is element e's
+    float2 x[EI / 2];
+    unpack(u, x, (const TI*)nullptr);
 #pragma unroll
     for (int i = 0; i < EI / 2; ++i) {
-      const float2 t = tc::ffma2(x[i], c2, nb);
-      const float2 d = tc::fmul2(make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y)), g2);
+      if (!kKeepPower) {
+        const float2 t = tc::ffma2(x[i], c2, nb);
+        x[i] = make_float2(tc::fast_exp2(t.x), tc::fast_exp2(t.y));
+      }
+      const float2 d = tc::fmul2(x[i], g2);
       v[2 * i] = d.x;
       v[2 * i + 1] = d.y;
     }
     const unsigned to = (unsigned)(token - e);
-    if (OP != kDistill && to < (unsigned)EI) {
+    if (!kList && to < (unsigned)EI) {
 #pragma unroll
       for (int i = 0; i < EI; ++i)
         if (to == (unsigned)i) v[i] += hot;
     }
   };
-  if ((uintptr_t)(dz + e_org) % (EI * sizeof(TO)) == 0) {
-    // the pieces' places in dz are aligned: every thread its own pieces
-    const int k0 = tid < f0 ? 1 : 0, k1 = owner && tid < f1 ? (f1 - tid + NT - 1) / NT : 0;
-#pragma unroll 2
-    for (int k = k0; k < k1; ++k) {
-      const int e = e_org + (tid + k * NT) * EI;
-      float2 x[EI / 2];
-      float v[EI];
-      unpack(at[k * NT], x, (const TI*)nullptr);
-      values(x, v, e);
-      store_n(dz + e, v);
-    }
-    // the pieces in part outside the row
-    auto in_part = [&](int i) {
-      const int e = e_org + i * EI;
-      float2 x[EI / 2];
-      float v[EI];
-      unpack(((const uint4*)dyn)[i], x, (const TI*)nullptr);
-      values(x, v, e);
+  auto give = [&](int e, const uint4 (&u)[U]) {  // a group that lies in the row, aligned
 #pragma unroll
-      for (int j = 0; j < EI; ++j)
-        if (e + j >= 0 && e + j < V) st(&dz[e + j], v[j]);
-    };
-    if (f0 == 1 && tid == 0 && np > 0) in_part(0);
-    if (f1 < np && f1 >= f0 && tid == f1 % NT) in_part(f1);
-  } else {
-    // units of dz straddle pieces: read across them
-    __syncthreads();
-    const int dph = (int)((uintptr_t)dz % (EI * sizeof(TO))) / (int)sizeof(TO);
-    const int u0 = (dph + e_lo + EI - 1) / EI, u1 = (dph + e_hi) / EI;
-#pragma unroll 2
-    for (int u = u0 + tid; u < u1; u += kThreadsOf<OP>) {
-      const int e = u * EI - dph;
-      const TI* in = image + (e - e_org);
-      float2 x[EI / 2];
+    for (int j = 0; j < U; ++j) {
       float v[EI];
-#pragma unroll
-      for (int i = 0; i < EI / 2; ++i) x[i] = make_float2(ld(&in[2 * i]), ld(&in[2 * i + 1]));
-      values(x, v, e);
-      store_n(dz + e, v);
+      values(u[j], e + j * (NT * EI), v);
+      store_n(dz + e + j * (NT * EI), v);
     }
-    const int ahead = u0 < u1 ? u0 * EI - dph : e_hi, behind = u0 < u1 ? u1 * EI - dph : e_hi;
-    auto one = [&](int e) {
-      const float d = c_out * tc::fast_exp2(fmaf(ld(&image[e - e_org]), f.c, -f.b));
-      st(&dz[e], OP != kDistill && e == token ? d + hot : d);
-    };
-    if (e_lo + tid < ahead) one(e_lo + tid);
-    if (behind + tid < e_hi) one(behind + tid);
+  };
+  auto give_one = [&](int k, uint4 u) {  // any piece
+    const int e = e_org + (tid + k * NT) * EI;
+    float v[EI];
+    values(u, e, v);
+    if (whole(k)) {
+      if (off == 0) store_n(dz + e, v);
+      else store_off(dz + e, v, off);
+    } else if (k < mine) {
+      store_elements(dz, e, V, EI, make_float4(v[0], v[1], v[2], v[3]),
+                     make_float4(v[EI - 4], v[EI - 3], v[EI - 2], v[EI - 1]));
+    }
+  };
+  if constexpr (kFits) {
+    if (owner) {
+      // groups [ga, gb) of this thread lie in the row
+      const int ga = tid < f0 ? 1 : 0, last = f1 - 1 - tid - (U - 1) * NT;
+      const int gb = off == 0 && last >= 0 ? last / (U * NT) + 1 : 0;
+      for (int g = ga; g < gb; ++g) {
+        uint4 u[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) u[j] = at[(g * U + j) * NT];
+        give(e_org + (tid + g * U * NT) * EI, u);
+      }
+#pragma unroll 1
+      for (int k = 0; k < mine; ++k) {
+        if (k == ga * U && gb > ga) k = gb * U;
+        if (k < mine) give_one(k, at[k * NT]);
+      }
+    }
+  } else if (owner) {
+    for (int g = 0, r = 0; g < groups; ++g) {
+      uint4 u[U];
+      if (kOnce) wait_group(g);
+      kept(g, r, u);
+      const int i = tid + g * U * NT;
+      if (off == 0 && i >= f0 && i + (U - 1) * NT < f1) {
+        give(e_org + i * EI, u);
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < U; ++j) give_one(g * U + j, j ? u[1] : u[0]);
+      }
+      if (kOnce) refill(g, r);
+      if (++r == ring) r = 0;
+    }
   }
-  if (OP == kDistill) {
+  if (kList || kTmem) {
+    tc::tc_fence_before();
     __syncthreads();
-    for (int k = tid; k < a.K; k += kThreadsOf<OP>)
+    tc::tc_fence_after();
+  }
+  if constexpr (kTmem)
+    if (warp == 0) free_columns<columns_of(S)>(s_tmem);
+  if (kList)
+#pragma unroll 1
+    for (int k = tid; k < a.K; k += THREADS)
       if (!(t_g[k] < 0.f))
         st(&dz[t_idx[k]], c_in * tc::fast_exp2(fmaf(t_z[k], f_in.c, -f_in.b)) - hot * t_g[k]);
-  }
 }
 
 // loss = scale * sum of l[0 .. n), in a fixed order, by NT threads.
@@ -769,18 +1018,18 @@ __global__ void __launch_bounds__(1024) k_scaled_sum(const float* l, int64_t n, 
   scaled_sum_of<1024>(l, n, scale, loss);
 }
 
-template <RowOp OP, typename TI, typename TO>
-__global__ void __launch_bounds__(kThreadsOf<OP>, kCtasPerSM<OP>) k_vocab_row(const RowArgs a) {
+template <RowOp OP, typename TI, typename TO, Shape S>
+__global__ void __launch_bounds__(kThreadsOf<OP, S>, kCtasPerSM<OP, S>) k_vocab_row(const RowArgs a) {
   if (OP == kLogpBwd) {
     // it has nothing to exchange: plain CTAs.  Last rows first: they are the
     // ones that the log-probabilities' pass has left in L2
     const unsigned C = (unsigned)a.cluster, r = blockIdx.x / C;
-    if (r == a.rows) return scaled_sum_of<kRowThreads>(a.sum_of, a.sum_n, a.scale, a.loss);
-    vocab_row<OP, TI, TO>(a, a.rows - 1 - r, (int)(blockIdx.x % C));
+    if (r == a.rows) return scaled_sum_of<owners_of(S)>(a.sum_of, a.sum_n, a.scale, a.loss);
+    vocab_row<OP, TI, TO, S>(a, a.rows - 1 - r, (int)(blockIdx.x % C));
   } else {
     uint32_t row;
     asm("mov.u32 %0, %%clusterid.x;" : "=r"(row));
-    vocab_row<OP, TI, TO>(a, row, (int)tc::cluster_ctarank());
+    vocab_row<OP, TI, TO, S>(a, row, (int)tc::cluster_ctarank());
   }
 }
 
@@ -803,8 +1052,8 @@ struct PairArgs {
   int normalize;
   float *pair_loss, *margin, *dlogp;
 };
-__global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_constant__ PairArgs a) {
-  __shared__ double s_red[kRowThreads / 32];
+__global__ void __launch_bounds__(kPairThreads) k_preference_pair(const __grid_constant__ PairArgs a) {
+  __shared__ double s_red[kPairThreads / 32];
   const int pair = blockIdx.x;
   const int64_t* off = a.off + 2 * pair;
   auto weight_of = [&](int64_t t) {
@@ -814,7 +1063,7 @@ __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_co
   double sum[2], len[2];
   for (int q = 0; q < 2; ++q) {
     double s = 0.0, n = 0.0;
-    for (int64_t t = off[q] + threadIdx.x; t < off[q + 1]; t += kRowThreads) {
+    for (int64_t t = off[q] + threadIdx.x; t < off[q + 1]; t += kPairThreads) {
       const float w = weight_of(t);
       if (w == 0.f) continue;
       s += (double)w * ((double)a.logp[t] - (a.ref_logp ? (double)a.ref_logp[t] : 0.0) +
@@ -836,7 +1085,7 @@ __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_co
   }
   for (int q = 0; q < 2; ++q) {
     const double g = (q ? -dm : dm) * a.beta * a.scale / (len[q] != 0.0 ? len[q] : 1.0);
-    for (int64_t t = off[q] + threadIdx.x; t < off[q + 1]; t += kRowThreads) {
+    for (int64_t t = off[q] + threadIdx.x; t < off[q + 1]; t += kPairThreads) {
       const float w = weight_of(t);
       a.dlogp[t] = w == 0.f ? 0.f : (float)(g * (double)w);
     }
@@ -844,10 +1093,11 @@ __global__ void __launch_bounds__(kRowThreads) k_preference_pair(const __grid_co
 }
 
 // ------------------------------------------------------------------- host
-// Shared memory of a list of K entries and its filter.
-constexpr int64_t list_bytes(int K) { return 16 * list_stride(K) + kFilterBits / 8; }
-constexpr int64_t kDynamicMost = kStageBytesMost + list_bytes(kMaxTeacherK);
-static_assert(kDynamicMost + 1536 <= 232448, "more shared memory than a CTA may have");
+// Shared memory of a list of K entries, without its bits.
+constexpr int64_t list_bytes(int K) { return 16 * list_stride(K); }
+constexpr int64_t kDynamicMost = 16 * owners_of(kAlone) * kRingMost + list_bytes(kMaxTeacherK) +
+                                 owners_of(kAlone) * (kRingMost + kMovedMost);  // (a bit per bf16 logit)
+static_assert(kDynamicMost + 2560 <= 232448, "more shared memory than a CTA may have");
 // Let a kernel use the shared memory it may need, once per device.
 void allow_shared_memory(const void* kern) {
   static std::mutex mu;
@@ -862,25 +1112,35 @@ void allow_shared_memory(const void* kern) {
   }
 }
 
-// How the rows are laid out over CTAs: as few of them per row as hold its
-// 16-byte pieces when three CTAs share an SM, more of them where the rows are
-// too few to occupy the SMs (down to 16 KB each), and at most kMaxCluster.
-// `once`: the pieces pass through a ring and need not fit.
+// How the rows are laid out over CTAs.  A row whose pieces are kept goes to
+// one narrow or held CTA or to as few wide ones as hold it; more of them where
+// the rows are too few to occupy the SMs (down to 16 KB each).
 struct Split {
   int cluster, share;  // CTAs per row; pieces per CTA
+  Shape shape;
+  int ring;            // places for pieces per owner
 };
-Split split_of(int64_t rows, int64_t vocab, int prec, int64_t lists, bool once) {
+Split split_of(int64_t rows, int64_t vocab, int prec, bool once, int passing) {
   // the pieces that a row touches wherever it starts
   const int64_t size = prec == DOP_BF16 ? 2 : 4, pieces = ceil_div(vocab * size + 16 - size, 16);
-  const int64_t fit = once ? 1 : ceil_div(16 * pieces, kCtaBytes - lists);
+  const int64_t narrow = kKept * owners_of(kNarrow), held = kHeldMost * owners_of(kHeld);
+  const int64_t wide = 2 * kKept * owners_of(kWide);
+  // (fp32 powers are kept, so that tensor memory costs nothing more)
+  const bool stay = prec == DOP_BF16 && pieces <= kMaxCluster * held;
+  const int64_t fit = once ? 1 : ceil_div(pieces, stay ? held : wide);
   const int64_t fill = std::min(ceil_div(3 * sm_count(), std::max<int64_t>(rows, 1)), ceil_div(pieces, 1024));
-  const int64_t C = std::min<int64_t>(std::max(fit, fill), kMaxCluster);
-  const int64_t share = ceil_div(pieces, C);
-  if (!once && 16 * share > kStageBytesMost)
-    throw Error(DOP_E_UNSUPPORTED, "vocab (" + std::to_string(vocab) + ") is above " +
-                                       std::to_string((C * kStageBytesMost - 16) / size + 1));
+  const int64_t C = std::min<int64_t>(std::max(fit, fill), kMaxCluster), share = ceil_div(pieces, C);
   if (rows * C >= INT32_MAX) throw Error(DOP_E_UNSUPPORTED, "too many rows for this vocab");
-  return {(int)C, (int)share};
+  if (once) return {(int)C, (int)share, kNarrow, passing};
+  const Shape shape = share <= narrow ? kNarrow : share <= held ? kHeld : share <= wide ? kWide : kAlone;
+  int64_t each = ceil_div(share, owners_of(shape));
+  if (columns_of(shape) > 0) each = round_up(each, 2);  // in groups of 2
+  if (each > kRingMost + kMovedMost)
+    throw Error(DOP_E_UNSUPPORTED,
+                "vocab (" + std::to_string(vocab) + ") is above " +
+                    std::to_string((C * owners_of(kAlone) * 16 * (kRingMost + kMovedMost) - 16) / size + 1));
+  const int most = shape == kAlone ? kRingMost : shape == kHeld ? kHeldMost : kKept;
+  return {(int)C, (int)share, shape, (int)std::min<int64_t>(each, most)};
 }
 
 // f(kernel's logit type, dlogits type)
@@ -911,16 +1171,35 @@ void launch(void (*kern)(A), const A& a, int64_t ctas, int threads, int64_t smem
 template <RowOp OP>
 void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t s) {
   if (rows == 0) return;
-  const int64_t lists = OP == kDistill ? list_bytes(a.K) : 0;
-  const Split sp = split_of(rows, a.V, prec, lists, OP == kLogp);
+  constexpr bool once = OP == kLogp || OP == kLogpBwd;
+  const Split sp = split_of(rows, a.V, prec, once, OP == kLogp ? kPassing : kKept);
+  a.rows = rows;
   a.cluster = sp.cluster;
   a.share = sp.share;
-  a.stage_bytes = 16 * (OP == kLogp ? std::min(sp.share, kRing * kOwnersOf<OP>) : sp.share);
-  a.rows = rows;
+  a.ring = sp.ring;
+  a.stage_bytes = 16 * owners_of(sp.shape) * sp.ring;
+  int64_t smem = a.stage_bytes;
+  if (has_list(OP)) {
+    const int64_t elements = (int64_t)sp.share * (prec == DOP_BF16 ? 8 : 4);
+    a.bit_words = (int)ceil_div(OP == kDistillRest ? elements : (int64_t)kFilterBits, 32);
+    smem += list_bytes(a.K) + 4 * a.bit_words;
+  }
+  if (sp.shape == kAlone) smem = std::max(smem, kAloneBytes);
   const int64_t ctas = rows * a.cluster + (a.sum_of ? 1 : 0);
+  const int cluster = OP == kLogpBwd ? 1 : a.cluster;
   by_types(prec, grad_prec, a.dz != nullptr, [&](auto ti, auto to) {
-    launch(k_vocab_row<OP, decltype(ti), decltype(to)>, a, ctas, kThreadsOf<OP>,
-           a.stage_bytes + lists, OP == kLogpBwd ? 1 : a.cluster, s);
+    using TI = decltype(ti);
+    using TO = decltype(to);
+    auto go = [&](auto shape) {
+      constexpr Shape S = decltype(shape)::value;
+      launch(k_vocab_row<OP, TI, TO, S>, a, ctas, kThreadsOf<OP, S>, smem, cluster, s);
+    };
+    if constexpr (!once) {
+      if (sp.shape == kAlone) return go(std::integral_constant<Shape, kAlone>{});
+      if (sp.shape == kWide) return go(std::integral_constant<Shape, kWide>{});
+      if (sp.shape == kHeld) return go(std::integral_constant<Shape, kHeld>{});
+    }
+    go(std::integral_constant<Shape, kNarrow>{});
   });
 }
 
@@ -931,7 +1210,7 @@ void check_rows(int64_t rows, int64_t vocab, int prec, const void* z, int64_t ld
   DOP_REQUIRE(rows >= 0 && rows <= INT32_MAX, "rows must lie in [0, 2^31)");
   DOP_REQUIRE(vocab >= 1 && vocab <= INT32_MAX, "vocab must lie in [1, 2^31)");
   DOP_REQUIRE(prec == DOP_F32 || prec == DOP_BF16, "unknown precision");
-  split_of(rows, vocab, prec, 0, false);
+  split_of(rows, vocab, prec, false, 0);
   DOP_REQUIRE(ld >= vocab, "the logits' row stride is smaller than vocab");
   DOP_REQUIRE(z || rows == 0, "null logits");
   DOP_REQUIRE((uintptr_t)z % elem_bytes(prec) == 0, "misaligned logits");
@@ -1103,7 +1382,7 @@ int dop_preference_loss_grad(int64_t rows, int64_t vocab, int precision, const v
       pa.pair_loss = pair_loss + p0;
       pa.margin = margin + p0;
       pa.dlogp = dlogp;
-      k_preference_pair<<<(unsigned)n, kRowThreads, 0, s>>>(pa);
+      k_preference_pair<<<(unsigned)n, kPairThreads, 0, s>>>(pa);
       DOP_CHECK_CUDA(cudaGetLastError());
     }
     if (!dlogits || rows == 0) return scaled_sum(pair_loss, pairs, scale, loss, s);
@@ -1143,7 +1422,8 @@ int dop_distill_loss_grad(int64_t rows, int64_t vocab, int precision, const void
     a.row_loss = row_loss;
     a.dz = dlogits;
     a.ldd = ldd;
-    launch_rows<kDistill>(a, rows, precision, grad_precision, as_stream(stream));
+    (teacher_lse ? launch_rows<kDistillRest> : launch_rows<kDistill>)(a, rows, precision, grad_precision,
+                                                                      as_stream(stream));
     scaled_sum(row_loss, rows, scale, loss, as_stream(stream));
   });
 }

@@ -109,7 +109,7 @@ def test_own_refusals(name, over):
 def test_unsupported_sizes():
     refused("dop_distill_loss_grad", code=-4, k=1025)
     for name in EVERY:
-        for prec, most in ((DOP_F32, 409_597), (DOP_BF16, 819_193)):
+        for prec, most in ((DOP_F32, 851_965), (DOP_BF16, 1_703_929)):
             refused(name, code=-4, prec=prec, gprec=prec, vocab=most + 1, ld=most + 1, ldd=most + 1)
 
 

@@ -90,7 +90,7 @@ def onehot(tokens, vocab, live):
 
 # ------------------------------------------------------------------ inputs
 SHAPES = [(1, 1), (3, 2), (5, 7), (1, 31), (4, 32), (2, 255), (3, 1000), (7, 4097), (2, 32000),
-          (1, 50001), (3, 131073)]
+          (1, 50001), (3, 131073), (500, 17), (450, 9001), (450, 20011), (446, 33003), (1, 700001)]
 LAYOUT = [(0, 0), (3, 1), (16, 0)]
 
 
@@ -279,6 +279,44 @@ def test_policy_branches(cuda):
     check("row_loss", r.row_loss, -adv, adv.abs().double() * 40 * U)
 
 
+FAR = [(2, 300), (1, 40007), (1, 300001)]  # a row on one CTA, and on several
+
+
+def far_rows(vocab, dtype, seed):
+    """Rows whose sums cannot be taken relative to their first elements: far
+    smaller ones ahead of a late maximum, all of the type's lowest value but
+    a few equal ones a little above it, all far, and a late entry near the
+    type's largest value."""
+    _, z = make_logits(5, vocab, dtype, 1, 0, seed=seed)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z[0] -= 300.0
+    z[0, -3] = 150.0
+    z[1] = low
+    z[1, vocab // 2::7] = low * 0.75
+    z[2] = low
+    z[3, -2] = high * 0.5
+    z[4, :-5] = low
+    return z
+
+
+@pytest.mark.parametrize("rows,vocab", FAR)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+def test_policy_far_rows(cuda, rows, vocab, dtype, grad):
+    z = far_rows(vocab, dtype, 23)
+    tokens = torch.tensor([vocab - 3, vocab // 2, 5, vocab - 2, vocab - 4], device="cuda")
+    x = torch.log_softmax(z.double(), 1)
+    logp = x.gather(1, tokens[:, None])[:, 0].float()
+    adv = torch.tensor([1.0, -0.5, 0.7, 1.3, 2.0], device="cuda")
+    ref = logp + 0.1
+    e = policy_reference(z, tokens, logp, adv, ref, None, 1.0, 0.2, 0.2, 0.1, 0.5)
+    # rel_of() counts the far logits as 0: their powers are exact
+    r = losses.policy_loss(z, tokens, logp, adv, ref_logp=ref, kl_coef=0.1, scale=0.5, grad_dtype=grad)
+    check_policy(r, e, 0.5, grad)
+    # the log-probability and the sum alone agree with it
+    got, lse = losses.token_logp(z, tokens)
+    check("logp", got, e["logp"], e["tol_logp"] + last(e["logp"], F32))
+
+
 # -------------------------------------------------------------- preference
 def preference_reference(z, tokens, off, ref_logp, weight, tau, beta, eps, norm, scale):
     rows, V = z.shape
@@ -438,7 +476,8 @@ def teacher(z, k, tau, seed, tail):
 
 @pytest.mark.parametrize("rows,vocab,k", [(1, 1, 1), (3, 2, 1), (5, 7, 3), (4, 32, 32), (2, 255, 100),
                                           (3, 1000, 1), (7, 4097, 64), (2, 32000, 128), (1, 50001, 1000),
-                                          (3, 131073, 17)])
+                                          (3, 131073, 17), (500, 17, 4), (450, 9001, 20), (450, 20011, 33),
+                                          (446, 33003, 64), (1, 700001, 50)])
 @pytest.mark.parametrize("pad,shift", LAYOUT)
 @pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
 @pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
@@ -509,6 +548,32 @@ def test_distill_extreme_rows(cuda):
     keep = [0, 2, 3]
     check("row_loss", r.row_loss[keep], e["row"][keep], (e["size"] * (e["rel"] + 8 * U) + last(e["row"], F32))[keep])
     check("dlogits", r.dlogits[keep], e["dlogits"][keep], (e["tol"] + last(e["dlogits"], F32))[keep])
+
+
+@pytest.mark.parametrize("rows,vocab", FAR)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+@pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
+def test_distill_far_rows(cuda, rows, vocab, dtype, grad, tail):
+    z = far_rows(vocab, dtype, 63)
+    index, top, tlse = teacher(z, 40, 1.0, 64, tail)
+    index[0, 0] = vocab - 3
+    index[1] = vocab // 2 + 7 * torch.arange(40, dtype=torch.int32, device="cuda") % (vocab // 2)
+    index[3, 0] = vocab - 2
+    keep = [0, 2] if tail else [0, 1, 2, 3]
+    for row in keep:  # (a far listed maximum leaves the others nothing: an infinite loss)
+        lp = torch.log_softmax(z[row].double(), 0)[index[row].long()]
+        top[row] = torch.where(lp > -80, top[row], torch.full_like(top[row], -math.inf))
+    if tail:
+        here = torch.logsumexp(top, 1)
+        tlse = torch.where(here > -50, here, torch.zeros_like(here)) + 0.2
+    rows_ = [r for r in keep if bool((top[r] > -math.inf).any())]
+    zz, ii, tt = z[rows_].clone(), index[rows_].contiguous(), top[rows_].contiguous()
+    tl = tlse[rows_].contiguous() if tail else None
+    e = distill_reference(zz, ii, tt, tl, None, 1.0, 1.0)
+    r = losses.distill_loss(zz, ii, tt, teacher_lse=tl, scale=1.0, grad_dtype=grad)
+    fine = torch.isfinite(e["row"])
+    check("row_loss", r.row_loss[fine], e["row"][fine], (e["size"] * (e["rel"] + 8 * U) + last(e["row"], F32))[fine])
+    check("dlogits", r.dlogits[fine], e["dlogits"][fine], (e["tol"] + last(e["dlogits"], grad))[fine])
 
 
 # -------------------------------------------------- gradient by differences
