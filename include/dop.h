@@ -316,16 +316,20 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  * no counterpart in the crate.  Conventions of all of them:
  *
  *   - x = z / temperature (between 2^-16 and 2^16), lse = log sum exp x,
- *     p = exp(x - lse).  Row r starts at logits + r * ld elements (ld >= vocab).  `precision` is the logits'
- *     type; dlogits has `grad_precision`: DOP_BF16, or DOP_F32 for fp32 logits.
- *     dlogits may be the logits' own memory when type and stride are the same
- *     (ldd == ld); any other overlap is refused.  dlogits is ASSIGNED, all of
- *     its rows x vocab elements and nothing between the rows; dlogits NULL
- *     computes the loss alone (not in dop_token_logp_backward).
+ *     p = exp(x - lse).  Row r starts at logits + r * ld elements (ld >= vocab);
+ *     a row and the matrices need the alignment of an element alone.
+ *     `precision` is the logits' type; dlogits has `grad_precision`: DOP_BF16,
+ *     or DOP_F32 for fp32 logits.  dlogits may be the logits' own memory when
+ *     type and stride are the same (ldd == ld); any other overlap is refused.
+ *     dlogits is ASSIGNED, all of its rows x vocab elements and nothing
+ *     between the rows; dlogits NULL computes the loss alone (not in
+ *     dop_token_logp_backward).  vocab is at most 851,965 (fp32 logits) or
+ *     1,703,929 (bf16): DOP_E_UNSUPPORTED above.
  *   - Sums and statistics are fp32 or wider, a row's scalars and the sums over
  *     rows fp64, all in a fixed order: equal inputs in equally aligned rows
- *     (address modulo 16) give equal bytes.  No call allocates, synchronises or keeps anything: all of them
- *     can be captured in a graph, and calls on different streams share nothing.
+ *     (address modulo 16) give equal bytes.  No call allocates, synchronises
+ *     or keeps anything: all of them can be captured in a graph, and calls on
+ *     different streams share nothing.
  *   - weight [rows] (NULL: 1) is a mask and a factor.  A row whose weight is 0,
  *     or whose token lies outside [0, vocab), is skipped: its logits are not
  *     read, its outputs and its row of dlogits are 0.
@@ -386,7 +390,8 @@ int dop_preference_loss_grad(int64_t rows, int64_t vocab, int precision, const v
  * temperature, q_k = exp(top_logit_k / temperature - teacher_lse) and what
  * both distributions hold outside the row's entries is one more class:
  * q_r = max(0, 1 - sum q), p_r = the sum of p there (none when the entries
- * are the whole vocabulary).  A row without entries has loss 0. */
+ * are the whole vocabulary).  A row without entries has loss 0.  Where the
+ * student has no probability for a class that q holds, the loss is infinite. */
 int dop_distill_loss_grad(int64_t rows, int64_t vocab, int precision, const void* logits,
                           int64_t ld, int64_t top_k, const int32_t* top_index,
                           const float* top_logit, const float* teacher_lse, const float* weight,

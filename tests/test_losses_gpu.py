@@ -317,6 +317,39 @@ def test_policy_far_rows(cuda, rows, vocab, dtype, grad):
     check("logp", got, e["logp"], e["tol_logp"] + last(e["logp"], F32))
 
 
+GAPS = [30.0, 43.0, 46.0, 60.0, 86.0, 88.0, 91.0, 97.0, 104.0]
+
+
+def uneven_rows(vocab, dtype, seed):
+    """Rows of which a third of the 16-byte pieces (in the first three fifths)
+    lie GAPS below the rest, so that what a thread meets first says little of
+    what it meets later, and below nothing of what another meets."""
+    _, z = make_logits(2 * len(GAPS), vocab, dtype, seed=seed, std=1.0)
+    i = torch.arange(vocab, device="cuda")
+    low = (i // (16 // z.element_size()) % 3 == 0) & (i < vocab * 3 // 5)
+    gap = torch.tensor(GAPS, device="cuda")
+    z[:len(GAPS)] -= (low * gap[:, None]).to(dtype)
+    z[len(GAPS):, vocab * 9 // 10] += gap.to(dtype)
+    return z
+
+
+UNEVEN = [300, 9001, 33003, 300001]
+
+
+@pytest.mark.parametrize("vocab", UNEVEN)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+def test_policy_uneven_rows(cuda, vocab, dtype, grad):
+    z = uneven_rows(vocab, dtype, 27)
+    tokens = tokens_of(z.shape[0], vocab, 28)
+    check_logp(z, tokens, None, 1.0, *losses.token_logp(z, tokens))
+    old, adv, ref = policy_inputs(z, tokens, 1.0, 29, 0.2, 0.2)
+    e = policy_reference(z, tokens, old, adv, ref, None, 1.0, 0.2, 0.2, 0.1, 0.5)
+    # of probabilities below 2^-62 fp32 need hold nothing
+    e["tol_dz"] = e["tol_dz"] + e["dlogits"].abs().amax(1, keepdim=True) * 2.0 ** -60
+    r = losses.policy_loss(z, tokens, old, adv, ref_logp=ref, kl_coef=0.1, scale=0.5, grad_dtype=grad)
+    check_policy(r, e, 0.5, grad)
+
+
 # -------------------------------------------------------------- preference
 def preference_reference(z, tokens, off, ref_logp, weight, tau, beta, eps, norm, scale):
     rows, V = z.shape
@@ -574,6 +607,18 @@ def test_distill_far_rows(cuda, rows, vocab, dtype, grad, tail):
     fine = torch.isfinite(e["row"])
     check("row_loss", r.row_loss[fine], e["row"][fine], (e["size"] * (e["rel"] + 8 * U) + last(e["row"], F32))[fine])
     check("dlogits", r.dlogits[fine], e["dlogits"][fine], (e["tol"] + last(e["dlogits"], grad))[fine])
+
+
+@pytest.mark.parametrize("vocab", UNEVEN)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+@pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
+def test_distill_uneven_rows(cuda, vocab, dtype, grad, tail):
+    z = uneven_rows(vocab, dtype, 67)
+    index, top, tlse = teacher(z, 30, 1.0, 68, tail)
+    e = distill_reference(z, index, top, tlse, None, 1.0, 1.0)
+    # of probabilities below 2^-62 fp32 need hold nothing
+    e["tol"] = e["tol"] + e["dlogits"].abs().amax(1, keepdim=True) * 2.0 ** -60
+    check_distill(losses.distill_loss(z, index, top, teacher_lse=tlse, scale=1.0, grad_dtype=grad), e, 1.0, grad)
 
 
 # -------------------------------------------------- gradient by differences
