@@ -621,6 +621,25 @@ def test_distill_uneven_rows(cuda, vocab, dtype, grad, tail):
     check_distill(losses.distill_loss(z, index, top, teacher_lse=tlse, scale=1.0, grad_dtype=grad), e, 1.0, grad)
 
 
+@pytest.mark.parametrize("dtype,grad,vocab", [(F32, F32, 851965), (F32, BF16, 851965), (BF16, BF16, 1703929)],
+                         ids=IDS)
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_largest_vocabulary(cuda, dtype, grad, vocab, shift):
+    """The longest rows there may be, from addresses that make them touch the
+    most 16-byte pieces, with the longest list."""
+    _, z = make_logits(2, vocab, dtype, 2, shift, seed=71)
+    tokens = torch.tensor([vocab - 1, 0], device="cuda")
+    check_logp(z, tokens, None, 1.0, *losses.token_logp(z, tokens))
+    old, adv, ref = policy_inputs(z, tokens, 1.0, 72, 0.2, 0.2)
+    e = policy_reference(z, tokens, old, adv, ref, None, 1.0, 0.2, 0.2, 0.1, 0.5)
+    check_policy(losses.policy_loss(z, tokens, old, adv, ref_logp=ref, kl_coef=0.1, scale=0.5, grad_dtype=grad),
+                 e, 0.5, grad)
+    for tail in (False, True):
+        index, top, tlse = teacher(z, 1024, 1.0, 73, tail)
+        e = distill_reference(z, index, top, tlse, None, 1.0, 1.0)
+        check_distill(losses.distill_loss(z, index, top, teacher_lse=tlse, scale=1.0, grad_dtype=grad), e, 1.0, grad)
+
+
 # -------------------------------------------------- gradient by differences
 @pytest.mark.parametrize("which", ["logp", "policy", "preference", "distill", "distill_tail"])
 def test_gradient_against_differences(cuda, which):
@@ -724,6 +743,28 @@ def test_other_streams_and_two_at_once(cuda):
         got[0].append(every(*sets[0], stream=one))
         with torch.cuda.stream(two):
             got[1].append(every(*sets[1]))
+    torch.cuda.synchronize()
+    for a, runs in zip(alone, got):
+        for r in runs:
+            assert all(torch.equal(x, y) for x, y in zip(a, r))
+
+
+def test_rows_of_every_shape_at_once(cuda):
+    """Rows kept in shared memory, in tensor memory and over clusters of CTAs,
+    on four streams at once."""
+    sets = []
+    for rows, vocab, dtype in ((600, 20011, BF16), (300, 33003, F32), (200, 131073, F32), (20, 700001, BF16)):
+        _, z = make_logits(rows, vocab, dtype, seed=vocab + 9)
+        sets.append((z, teacher(z, 16, 1.0, 110, True)))
+    call = lambda z, t: losses.distill_loss(z, t[0], t[1], teacher_lse=t[2])
+    alone = [call(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for _ in range(3):
+        for s, stream, g in zip(sets, streams, got):
+            with torch.cuda.stream(stream):
+                g.append(call(*s))
     torch.cuda.synchronize()
     for a, runs in zip(alone, got):
         for r in runs:
