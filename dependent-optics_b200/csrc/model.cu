@@ -148,6 +148,7 @@ struct Model {
   template <typename Act>
   void forward(const Act* P, const int64_t* tokens, float* logits_to, cudaStream_t s) {
     const int64_t D = cfg.dim, V = cfg.vocab, L = cfg.layers;
+    have_tape = false;
     k_embed<Act><<<(unsigned)T, 256, 0, s>>>(P + embed, tokens, (int)D, acts[0]);
     DOP_LAUNCHED(launches);
     for (int64_t l = 0; l < L; ++l)
