@@ -20,14 +20,14 @@
 // B200 (6.46 TB/s of measured copy bandwidth), of the bytes read and written
 // once:
 //
-//   log-probabilities, 16384 x 32000 bf16, a fifth skipped          146 us  0.89
-//   their adjoint, 4095 x 50001 fp32 to bf16                        210 us  0.90
-//   policy loss, 8192 x 32000 fp32 to bf16, a quarter skipped       236 us  0.86
-//   policy loss, 3001 x 100003 bf16 (rows on odd addresses)         259 us  0.72
-//   preference loss, 16384 x 32000 bf16, three tenths skipped       405 us  0.68
-//     (the margins come between two readings of the logits: 0.96 of three passes)
-//   distillation from 64 logits, 32768 x 32000 bf16                 843 us  0.77
-//   with a class for the rest, 128 logits, 2047 x 128000 fp32       413 us  0.79
+//   log-probabilities, 16384 x 32000 bf16, a fifth skipped          145 us  0.90
+//   their adjoint, 4095 x 50001 fp32 to bf16                        209 us  0.91
+//   policy loss, 8192 x 32000 fp32 to bf16, a quarter skipped       235 us  0.86
+//   policy loss, 3001 x 100003 bf16 (rows on odd addresses)         252 us  0.74
+//   preference loss, 16384 x 32000 bf16, three tenths skipped       409 us  0.67
+//     (the margins come between two readings of the logits: 0.95 of three passes)
+//   distillation from 64 logits, 32768 x 32000 bf16                 840 us  0.77
+//   with a class for the rest, 128 logits, 2047 x 128000 fp32       420 us  0.77
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -188,19 +188,7 @@ __device__ __forceinline__ void copy_piece(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Wait until at most `n` of this thread's copy groups are under way.
-__device__ __forceinline__ void copy_wait(int n) {
-  switch (n) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    case 4: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
-    case 5: asm volatile("cp.async.wait_group 5;" ::: "memory"); break;
-    case 6: asm volatile("cp.async.wait_group 6;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 7;" ::: "memory"); break;
-  }
-}
+// Wait until at most N of this thread's copy groups are under way.
 template <int N>
 __device__ __forceinline__ void copy_wait_for() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -1145,7 +1133,13 @@ void allow_shared_memory(const void* kern) {
 
 // How the rows are laid out over CTAs.  A row whose pieces are kept goes to
 // one narrow or held CTA or to as few wide ones as hold it; more of them where
-// the rows are too few to occupy the SMs (down to 16 KB each).
+// the rows are too few to occupy the SMs (down to 16 KB each).  Both sides, in
+// us: narrow against held for 16384 x 16001 bf16, policy loss 202 / 260,
+// distillation 254 / 344; one held CTA against two narrow ones for 32768 x
+// 32000 bf16, distillation 808 / 883, and against a wide one, 8192 rows, 221 /
+// 237; a wide CTA against four narrow ones for 8192 x 32000 fp32, policy loss
+// 223 / 258; two wide ones against three held ones for 3001 x 100003 bf16,
+// policy loss 250 / 259, and 3000 rows distilled with a rest class 275 / 407.
 struct Split {
   int cluster, share;  // CTAs per row; pieces per CTA
   Shape shape;
