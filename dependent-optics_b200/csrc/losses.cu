@@ -83,8 +83,10 @@ struct RowArgs {
   double inv_tau;
   float c;       // log2(e) / tau
   int64_t rows, in_lo, in_hi;  // rows outside [in_lo, in_hi) are skipped
-  const float* sum_of;  // the preference loss: scale times the sum of these,
-  int64_t sum_n;        // taken with the adjoint
+  // the preference loss, taken with the adjoint: loss (null: none) = scale
+  // times the sum of sum_of[0 .. sum_n)
+  const float* sum_of;
+  int64_t sum_n;
   float* loss;
   int cluster;      // CTAs per row
   int share;         // 16-byte pieces of a row a CTA has
@@ -1208,7 +1210,7 @@ void launch_rows(RowArgs a, int64_t rows, int prec, int grad_prec, cudaStream_t 
     smem += list_bytes(a.K) + 4 * a.bit_words;
   }
   if (sp.shape == kAlone) smem = std::max(smem, kAloneBytes);
-  const int64_t ctas = rows * a.cluster + (a.sum_of ? 1 : 0);
+  const int64_t ctas = rows * a.cluster + (OP == kLogpBwd && a.loss ? 1 : 0);  // (one for the sum)
   const int cluster = OP == kLogpBwd ? 1 : a.cluster;
   by_types(prec, grad_prec, a.dz != nullptr, [&](auto ti, auto to) {
     using TI = decltype(ti);
