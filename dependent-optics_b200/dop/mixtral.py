@@ -302,6 +302,8 @@ class Model:
         h = C.c_void_p()
         check(lib().dop_model_create(C.byref(cfg.to_c()), batch, seq, precision, C.byref(h)))
         self._h = h
+        import torch
+        self.device = torch.device("cuda", torch.cuda.current_device())
         self.n_params = int(lib().dop_model_parameter_count(h))
 
     def close(self) -> None:
@@ -324,14 +326,38 @@ class Model:
                                                stream_ptr(stream)))
         return LossGrad(loss, grad, logits)
 
+    def _check(self, *operands):
+        """Refuses operands (tensor, name, types, shape) that a pointer would
+        not show to be of another type, size, layout or device than the call
+        reads or writes (a shape that is a number: that many elements in any)."""
+        import torch
+        for t, name, types, shape in operands:
+            if (not isinstance(t, torch.Tensor) or t.dtype not in types or not t.is_contiguous()
+                    or (t.numel() if isinstance(shape, int) else t.shape) != shape):
+                raise _lib.DopError(-1, f"invalid argument: {name} must be a contiguous tensor of "
+                                        f"{' or '.join(map(str, types))} and size {shape}")
+            if t.device != self.device:
+                raise _lib.DopError(-1, f"invalid argument: {name} must be on the model's device")
+
+    def _inputs(self, params, tokens):
+        import torch
+        act = torch.float32 if self.precision == DOP_F32 else torch.bfloat16
+        return ((params, "params", (act,), self.n_params),
+                (tokens, "tokens", (torch.int64,), self.batch * self.seq))
+
     def forward(self, params, tokens, logits=None, stream=None):
         """The get: logits fp32 [batch*seq, vocab]; the residual stays in the
-        handle for `backward`.  stream None is the current stream."""
+        handle for `backward`.  Work goes to `stream`, or to the current stream
+        when it is None.  Every tensor is contiguous and on the device the
+        model was made on: params [n_params] in the model's precision, tokens
+        int64 [batch*seq] (in any shape), `logits` (written) as above."""
         import torch
+        f32, shape = torch.float32, (self.batch * self.seq, self.cfg.vocab)
+        out = () if logits is None else ((logits, "logits", (f32,), shape),)
+        self._check(*self._inputs(params, tokens), *out)
         stream = stream or torch.cuda.current_stream(params.device)
         if logits is None:
-            logits = torch.empty(self.batch * self.seq, self.cfg.vocab, dtype=torch.float32,
-                                 device=params.device)
+            logits = torch.empty(shape, dtype=f32, device=self.device)
         check(lib().dop_model_forward(self._h, ptr(params), ptr(tokens), ptr(logits),
                                       stream_ptr(stream)))
         return logits
@@ -339,17 +365,17 @@ class Model:
     def backward(self, params, tokens, dlogits, grad=None, stream=None):
         """The put: the parameter adjoint of the last forward's logits from
         their cotangent dlogits [batch*seq, vocab] (contiguous; fp32, or bf16
-        for a bf16 model), e.g. one of `dop.losses`.  `grad` is overwritten.
-        stream None is the current stream."""
+        for a bf16 model), e.g. one of `dop.losses`.  `grad` (fp32 [n_params])
+        is overwritten.  Streams, params and tokens as in `forward`."""
         import torch
+        f32, shape = torch.float32, (self.batch * self.seq, self.cfg.vocab)
+        kinds = (f32,) if self.precision == DOP_F32 else (f32, torch.bfloat16)
+        out = () if grad is None else ((grad, "grad", (f32,), self.n_params),)
+        self._check(*self._inputs(params, tokens), (dlogits, "dlogits", kinds, shape), *out)
         stream = stream or torch.cuda.current_stream(params.device)
-        if (dlogits.shape != (self.batch * self.seq, self.cfg.vocab) or not dlogits.is_contiguous()
-                or dlogits.dtype not in (torch.float32, torch.bfloat16)):
-            raise _lib.DopError(-1, "invalid argument: dlogits must be a contiguous fp32 or bf16 "
-                                    "tensor [batch*seq, vocab]")
         if grad is None:
-            grad = torch.empty(self.n_params, dtype=torch.float32, device=params.device)
-        prec = DOP_F32 if dlogits.dtype is torch.float32 else DOP_BF16
+            grad = torch.empty(self.n_params, dtype=f32, device=self.device)
+        prec = DOP_F32 if dlogits.dtype is f32 else DOP_BF16
         check(lib().dop_model_backward(self._h, ptr(params), ptr(tokens), prec, ptr(dlogits),
                                        ptr(grad), stream_ptr(stream)))
         return grad

@@ -6,8 +6,8 @@ import pytest
 import torch
 
 from dop import losses
-from dop._lib import DOP_F32, check as ok, lib
-from test_losses_gpu import tokens_of
+from dop._lib import DOP_F32, DopError, check as ok, lib
+from test_losses_gpu import demo, tokens_of
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,25 @@ def test_preference_without_pairs(cuda, rows, off, grad):
     assert (dz == (0.0 if grad else 7.0)).all()
     r = losses.preference_loss(z, tokens, off, grad=grad)
     assert float(r.loss) == 0.0 and r.pair_loss.shape == (0,)
+
+
+# ------------------------------------------------ the model's get and put
+def test_model_operands(cuda):
+    """Outputs and inputs of another type, size, layout or device are refused
+    (tests/test_model_operands_cpu.py has each of them)."""
+    c, m, P, tokens, targets = demo(DOP_F32)
+    z = m.forward(P, tokens)
+    for bad in (z.bfloat16(), z[:-1].clone(), z.cpu(), z.t()):
+        with pytest.raises(DopError):
+            m.forward(P, tokens, logits=bad)
+        with pytest.raises(DopError):
+            m.backward(P, tokens, bad)
+    for bad in (P[:-1], P.bfloat16(), P.cpu()):
+        with pytest.raises(DopError):
+            m.backward(P, tokens, z, grad=bad)
+        with pytest.raises(DopError):
+            m.forward(bad, tokens)
+    with pytest.raises(DopError):
+        m.forward(P, tokens.int())
+    assert m.forward(P, tokens, logits=z) is z
+    m.close()
