@@ -326,10 +326,12 @@ class Model:
                                                stream_ptr(stream)))
         return LossGrad(loss, grad, logits)
 
-    def _check(self, *operands):
+    def _call(self, stream, *operands):
         """Refuses operands (tensor, name, types, shape) that a pointer would
         not show to be of another type, size, layout or device than the call
-        reads or writes (a shape that is a number: that many elements in any)."""
+        reads or writes (a shape that is a number: that many elements in any).
+        Returns a context in which the handle's device and the call's stream
+        are current: what the call allocates then belongs to that stream."""
         import torch
         for t, name, types, shape in operands:
             if (not isinstance(t, torch.Tensor) or t.dtype not in types or not t.is_contiguous()
@@ -338,6 +340,12 @@ class Model:
                                         f"{' or '.join(map(str, types))} and size {shape}")
             if t.device != self.device:
                 raise _lib.DopError(-1, f"invalid argument: {name} must be on the model's device")
+        if stream is None:
+            return torch.cuda.device(self.device)
+        if stream.device != self.device:
+            raise _lib.DopError(-1, "invalid argument: the stream belongs to another device than "
+                                    "the model")
+        return torch.cuda.stream(stream)
 
     def _inputs(self, params, tokens):
         import torch
@@ -354,12 +362,11 @@ class Model:
         import torch
         f32, shape = torch.float32, (self.batch * self.seq, self.cfg.vocab)
         out = () if logits is None else ((logits, "logits", (f32,), shape),)
-        self._check(*self._inputs(params, tokens), *out)
-        stream = stream or torch.cuda.current_stream(params.device)
-        if logits is None:
-            logits = torch.empty(shape, dtype=f32, device=self.device)
-        check(lib().dop_model_forward(self._h, ptr(params), ptr(tokens), ptr(logits),
-                                      stream_ptr(stream)))
+        with self._call(stream, *self._inputs(params, tokens), *out):
+            if logits is None:
+                logits = torch.empty(shape, dtype=f32, device=self.device)
+            check(lib().dop_model_forward(self._h, ptr(params), ptr(tokens), ptr(logits),
+                                          torch.cuda.current_stream().cuda_stream))
         return logits
 
     def backward(self, params, tokens, dlogits, grad=None, stream=None):
@@ -371,13 +378,13 @@ class Model:
         f32, shape = torch.float32, (self.batch * self.seq, self.cfg.vocab)
         kinds = (f32,) if self.precision == DOP_F32 else (f32, torch.bfloat16)
         out = () if grad is None else ((grad, "grad", (f32,), self.n_params),)
-        self._check(*self._inputs(params, tokens), (dlogits, "dlogits", kinds, shape), *out)
-        stream = stream or torch.cuda.current_stream(params.device)
-        if grad is None:
-            grad = torch.empty(self.n_params, dtype=f32, device=self.device)
-        prec = DOP_F32 if dlogits.dtype is f32 else DOP_BF16
-        check(lib().dop_model_backward(self._h, ptr(params), ptr(tokens), prec, ptr(dlogits),
-                                       ptr(grad), stream_ptr(stream)))
+        with self._call(stream, *self._inputs(params, tokens),
+                        (dlogits, "dlogits", kinds, shape), *out):
+            if grad is None:
+                grad = torch.empty(self.n_params, dtype=f32, device=self.device)
+            prec = DOP_F32 if dlogits.dtype is f32 else DOP_BF16
+            check(lib().dop_model_backward(self._h, ptr(params), ptr(tokens), prec, ptr(dlogits),
+                                           ptr(grad), torch.cuda.current_stream().cuda_stream))
         return grad
 
 

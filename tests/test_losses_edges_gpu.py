@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from dop import losses
-from dop._lib import DOP_F32, DopError, check as ok, lib
+from dop._lib import DOP_BF16, DOP_F32, DopError, check as ok, lib
 from test_losses_gpu import demo, tokens_of
 
 pytestmark = pytest.mark.gpu
@@ -37,7 +37,39 @@ def test_preference_without_pairs(cuda, rows, off, grad):
     assert float(r.loss) == 0.0 and r.pair_loss.shape == (0,)
 
 
-# ------------------------------------------------ the model's get and put
+# --------------------------------------------- the model's get and put, streams
+def pool_of(t):
+    """The stream that the allocator has t's memory for."""
+    for s in torch.cuda.memory_snapshot():
+        if s["address"] <= t.data_ptr() < s["address"] + s["total_size"]:
+            return s["stream"]
+    raise AssertionError("not the allocator's")
+
+
+@pytest.mark.parametrize("precision", [DOP_F32, DOP_BF16], ids=["f32", "bf16"])
+def test_model_on_another_stream(cuda, precision):
+    """The get and the put on a stream that is not current, given or entered:
+    the same bytes, in memory of that stream."""
+    c, m, P, tokens, targets = demo(precision)
+    want = m.forward(P, tokens)
+    g = losses.token_logp_backward(want, targets, losses.token_logp(want, targets)[1],
+                                   torch.ones(tokens.numel(), device="cuda"))
+    grad = m.backward(P, tokens, g)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    z = m.forward(P, tokens, stream=side)
+    d = m.backward(P, tokens, g, stream=side)
+    with torch.cuda.stream(side):
+        z2 = m.forward(P, tokens.view(2, -1))
+        d2 = m.backward(P, tokens.view(2, -1), g)
+    torch.cuda.synchronize()
+    for a, b in ((z, want), (z2, want), (d, grad), (d2, grad)):
+        assert torch.equal(a, b)
+    assert [pool_of(t) for t in (z, d, z2, d2)] == [side.cuda_stream] * 4
+    assert pool_of(want) == pool_of(grad) == torch.cuda.current_stream().cuda_stream
+    m.close()
+
+
 def test_model_operands(cuda):
     """Outputs and inputs of another type, size, layout or device are refused
     (tests/test_model_operands_cpu.py has each of them)."""
