@@ -113,24 +113,36 @@ struct RowArgs {
 // 2^(c z - b) with b = rint(c m), a whole number: one fused multiply-add an
 // element, no rounding of b, and sums with different b differ by exact powers
 // of two.  (c is log2(e) / tau rounded to fp32, for every term of a row alike:
-// a relative change of the temperature by at most 2^-24.)  b is held within
-// +-1e30.  Where c m would pass that, or a row is all of the type's lowest
-// value, two elements are equal or at least 2^60 apart: beyond 1e25 a row is
-// far, and its powers are taken of (z - m) 2^-40, which is exact.
-constexpr float kFar = 1e30f;
+// a relative change of the temperature by at most 2^-24.)
+//
+// From |c m| = 2^24 on fp32 has no whole number near c m (b would miss it by
+// up to half of its last digit, and the power at m itself would leave fp32);
+// such a maximum is far.  The powers are then 2^(c (z - m)), from elements
+// that m has been subtracted from: fp32 holds z - m to 2^-24 of it; in bf16
+// two elements that differ do so by 2^15 / c at least, which leaves the
+// smaller one nothing, and equal ones give 0.
+constexpr float kFar = 0x1p24f;
+constexpr float kBaseMost = 1e30f;  // (of a maximum of -inf)
 __device__ __forceinline__ float base_of(float m, float c) {
   constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: to a whole number without a conversion
-  return fminf(fmaxf((c * m + kRound) - kRound, -kFar), kFar);
+  return fminf(fmaxf((c * m + kRound) - kRound, -kBaseMost), kBaseMost);
 }
-__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > 1e25f && m != -INFINITY; }
+__device__ __forceinline__ bool is_far(float m, float c) {  // (+inf and NaN are)
+  return !(fabsf(c * m) < kFar) && m != -INFINITY;
+}
 struct Form {
-  float c, b;  // 2^(c z - b)
+  float c, b, m;  // 2^(c (z - m) - b)
 };
 __device__ __forceinline__ Form form_of(float m, float c) {
-  if (is_far(m)) return {0x1p-40f, m * 0x1p-40f};
-  return {c, base_of(m, c)};
+  if (is_far(m, c)) return {c, 0.f, m};
+  return {c, base_of(m, c), 0.f};
 }
-// A maximum and the sum of 2^(c z - b) of its form; nothing: {-inf, 0}.
+__device__ __forceinline__ float power(float z, const Form& f) {
+  return tc::fast_exp2(fmaf(z - f.m, f.c, -f.b));
+}
+// A maximum and a sum of powers; nothing: {-inf, 0}.  While the sums are put
+// together they are relative to base_of(m) (of a far row: no sum yet); the
+// row's, and those of listed entries, are of form_of(m).
 struct MaxSum {
   float m, s;
 };
@@ -139,24 +151,33 @@ __device__ __forceinline__ float warp_max_redux(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-// The warp's maximum and sum; the sum of a far row is not one yet.
+// What turns a sum relative to base_of(m) into one relative to that of `to` >= m.
+__device__ __forceinline__ float rebase(float m, float to, float c) {
+  return m == to ? 1.f : tc::fast_exp2(base_of(m, c) - base_of(to, c));
+}
+// The warp's maximum and sum, relative to its base.
 __device__ __forceinline__ MaxSum warp_join(MaxSum v, float c) {
   const float m = warp_max_redux(v.m);
   return {m, warp_sum(v.s * tc::fast_exp2(base_of(v.m, c) - base_of(m, c)))};
 }
-// What turns a sum relative to m into one relative to `to` >= m.
-__device__ __forceinline__ float rescale(float m, float to, float c) {
-  if (m == to) return 1.f;
-  if (is_far(m) || is_far(to)) return 0.f;
-  return tc::fast_exp2(base_of(m, c) - base_of(to, c));
-}
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
   const float m = fmaxf(a.m, b.m);
-  return {m, a.s * rescale(a.m, m, c) + b.s * rescale(b.m, m, c)};
+  return {m, a.s * rebase(a.m, m, c) + b.s * rebase(b.m, m, c)};
+}
+// c z where the powers of form_of(m) are 1 (exact: 48 bits).
+__device__ __forceinline__ double origin(float m, float c) {
+  return is_far(m, c) ? (double)c * (double)m : (double)base_of(m, c);
+}
+// What turns a sum of form_of(m) into one of form_of(to), to >= m.
+__device__ __forceinline__ float rescale(float m, float to, float c) {
+  if (m == to) return 1.f;
+  if (m == -INFINITY) return 0.f;
+  if (!is_far(m, c) && !is_far(to, c)) return tc::fast_exp2(base_of(m, c) - base_of(to, c));
+  return tc::fast_exp2((float)(origin(m, c) - origin(to, c)));
 }
 // (z - m) / tau, to which log(s) is to be taken from, in double.
 __device__ __forceinline__ double above(float z, float m, float c, double inv_tau) {
-  if (is_far(m)) return ((double)z - (double)m) * inv_tau;
+  if (is_far(m, c)) return ((double)z - (double)m) * inv_tau;
   return ((double)z * (double)c - (double)base_of(m, c)) * kLn2;
 }
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -208,6 +229,18 @@ __device__ __forceinline__ void unpack(uint4 u, float2* x, const bf16*) {
   x[1] = bf16x2(u.y);
   x[2] = bf16x2(u.z);
   x[3] = bf16x2(u.w);
+}
+// A piece less m (out of line: of far rows alone).
+__device__ __noinline__ uint4 minus(uint4 u, float m, const float*) {
+  return make_uint4(__float_as_uint(__uint_as_float(u.x) - m), __float_as_uint(__uint_as_float(u.y) - m),
+                    __float_as_uint(__uint_as_float(u.z) - m), __float_as_uint(__uint_as_float(u.w) - m));
+}
+__device__ __noinline__ uint4 minus(uint4 u, float m, const bf16*) {
+  auto word = [m](uint32_t w) {
+    const float2 x = bf16x2(w);
+    return tc::pack_bf16(x.x - m, x.y - m);
+  };
+  return make_uint4(word(u.x), word(u.y), word(u.z), word(u.w));
 }
 __device__ __forceinline__ uint32_t minus_inf_word(const float*) { return 0xff800000u; }
 __device__ __forceinline__ uint32_t minus_inf_word(const bf16*) { return 0xff80ff80u; }
@@ -529,7 +562,7 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       t.m = warp_max_redux(t.m);
       const Form f = form_of(t.m, a.c);
 #pragma unroll 1
-      for (int k = lane; k < a.K; k += 32) t.s += tc::fast_exp2(fmaf(t_q[k], f.c, -f.b));
+      for (int k = lane; k < a.K; k += 32) t.s += power(t_q[k], f);
       tl = ln(warp_sum(t.s));
     }
     double qs = 0.0, ql = 0.0;
@@ -599,14 +632,15 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     }
   };
   // a group whose maximum and sum have been taken
-  auto keep = [&](int g, int r, const uint4 (&u)[U]) {
+  // (shifted: less the maximum, so that they too are not what the ring holds)
+  auto keep = [&](int g, int r, const uint4 (&u)[U], bool shifted = false) {
     if (kOnce || !dz) return;
     if (g < moved) {
       if constexpr (kTmem) {
         __syncwarp();
         tmem_put(lane_tmem + (uint32_t)(g * 4 * U), u);
       }
-    } else if (kKeepPower) {
+    } else if (kKeepPower || shifted) {
 #pragma unroll
       for (int j = 0; j < U; ++j)
         if (!kFits || g * U + j < mine) at[(r * U + j) * NT] = u[j];
@@ -753,7 +787,7 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
         const Form f = form_of(listed.m, a.c);
 #pragma unroll 1
         for (int k = lane; k < a.K; k += 32)
-          if (!(t_g[k] < 0.f)) listed.s += tc::fast_exp2(fmaf(t_z[k], f.c, -f.b));
+          if (!(t_g[k] < 0.f)) listed.s += power(t_z[k], f);
         listed.s = warp_sum(listed.s);
         count = warp_sum(count);
       }
@@ -768,9 +802,10 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     }
     told();
     // A sum relative to first pieces is none when later elements pass them by
-    // 2^64, nor is one of far elements; then all is taken once more, relative
-    // to the maximum of the row.
-    auto not_one = [&](const MaxSum& v) { return is_far(v.m) || !(v.s < INFINITY); };
+    // 2^64, nor is one of a far maximum; then all is taken once more, relative
+    // to the maximum of the row, which is subtracted from what is kept where
+    // it is far.
+    auto not_one = [&](const MaxSum& v) { return is_far(v.m, a.c) || !(v.s < INFINITY); };
     if (OP == kLogp && C == 1 && warp != 0) {  // (which needs every warp)
       bool once_more = false;
       for (int i = 0; i < NW; ++i) once_more = once_more || not_one(s_rest[i]);
@@ -796,17 +831,20 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       for (int i = lane; i < C * NW; i += 32) m = fmaxf(m, s_again[i]);
       rest.m = warp_max_redux(m);
       const Form f = form_of(rest.m, a.c);
-      c2 = make_float2(f.c, f.c);
+      const bool far = is_far(rest.m, a.c);
       nb = make_float2(-f.b, -f.b);
-      my_base = base_of(rest.m, a.c);
+      my_base = f.b;
       s0 = s1 = make_float2(0.f, 0.f);
       if (owner)
 #pragma unroll 1
         for (int g = 0, r = 0; g < groups; ++g) {
           anew(g, u);
           without_listed(g, u);
+          if (far)
+#pragma unroll
+            for (int j = 0; j < U; ++j) u[j] = minus(u[j], f.m, (const TI*)nullptr);
           add(u);
-          keep(g, r, u);
+          keep(g, r, u, far);
           if (++r == ring) r = 0;
         }
       exchange(warp_sum(sum()), s_again + kMaxCluster * NW);
@@ -826,8 +864,12 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       listed.s = warp_sum(one.s * rescale(one.m, listed.m, a.c));
       count = warp_sum(count);
     }
-    all = kList ? join(rest, listed, a.c) : rest;
-    if (kList && is_far(all.m)) {
+    all = rest;
+    if (tail) {
+      all.m = fmaxf(rest.m, listed.m);
+      all.s = rest.s * rescale(rest.m, all.m, a.c) + listed.s * rescale(listed.m, all.m, a.c);
+    }
+    if (kList && is_far(all.m, a.c)) {
       // the sum of q (z - m) instead, which keeps its digits
       if (!owner) {
         qz = 0.0;
@@ -860,10 +902,10 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     const double l2 = (double)lse_in * kLog2e;
     hot = (float)((double)dlogp * a.inv_tau);
     if (fabsf(lse_in) > 1e25f) {
-      f = {0.f, 1e4f};
+      f = {0.f, 1e4f, 0.f};
       c_out = -hot;
     } else {
-      f = {a.c, (float)rint(l2)};
+      f = {a.c, (float)rint(l2), 0.f};
       c_out = -hot * tc::fast_exp2((float)((double)f.b - l2));
     }
   } else if (OP == kPolicy) {
@@ -894,7 +936,7 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     // outside the list relative to the largest logit there: the student's
     // mass outside may be too small to be held relative to the row's largest
     // (none at all: an infinite loss, and entries of probability 0)
-    c_out = rest.s == 0.f ? (all.s == 0.f ? NAN : 0.f)
+    c_out = rest.s == 0.f ? (all.s > 0.f ? 0.f : NAN)
                           : c_in * rescale(rest.m, all.m, a.c) -
                                 (q_rest > 0.f ? hot * q_rest / rest.s : 0.f);
     if (!owner && rank == 0 && lane == 0) {
@@ -903,13 +945,15 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
 #pragma unroll 1
       for (int i = 0; i < C; ++i) qz += s_qz[i];
       // sum of q (z / tau - lse), as above() has it of one z
-      const double x = is_far(all.m) ? qz * a.inv_tau
-                                     : (qz * (double)a.c - qs * (double)f_in.b) * kLn2;
+      const bool far = is_far(all.m, a.c);
+      const double x = far ? qz * a.inv_tau : (qz * (double)a.c - qs * (double)f_in.b) * kLn2;
       double l = s_q[1] - (x - qs * ls_all);
-      if (q_rest > 0.f)  // -log of the student's share outside the list
-        l += (double)q_rest *
-             ((double)logf(q_rest) + (ls_all - ls_rest) -
-              (above(0.f, all.m, a.c, a.inv_tau) - above(0.f, rest.m, a.c, a.inv_tau)));
+      if (q_rest > 0.f) {  // -log of the student's share outside the list
+        const double apart = far && is_far(rest.m, a.c)
+                                 ? ((double)all.m - (double)rest.m) * a.inv_tau
+                                 : (origin(all.m, a.c) - origin(rest.m, a.c)) * kLn2;
+        l += (double)q_rest * ((double)logf(q_rest) + (ls_all - ls_rest) + apart);
+      }
       a.row_loss[row] = (float)((double)w * l / (a.inv_tau * a.inv_tau));
     }
     if (!owner && !tail && dz) {
@@ -929,7 +973,7 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
   // ---- the adjoint
   // powers that were kept are relative to this thread's own base (each below
   // 2^64: where this factor underflows, what is lost is below 2^-62 of `hot`)
-  if (kKeepPower && !is_far(rest.m)) c_out *= tc::fast_exp2(my_base - f.b);
+  if (kKeepPower && !is_far(rest.m, a.c)) c_out *= tc::fast_exp2(my_base - f.b);
   const float2 c2 = make_float2(f.c, f.c), nb = make_float2(-f.b, -f.b);
   const float2 g2 = make_float2(c_out, c_out);
   const int off = (int)((uintptr_t)(dz + e_org) % (EI * sizeof(TO)));  // of every piece's place in dz
@@ -1017,7 +1061,7 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
 #pragma unroll 1
     for (int k = tid; k < a.K; k += THREADS)
       if (!(t_g[k] < 0.f))
-        st(&dz[t_idx[k]], c_in * tc::fast_exp2(fmaf(t_z[k], f_in.c, -f_in.b)) - hot * t_g[k]);
+        st(&dz[t_idx[k]], c_in * power(t_z[k], f_in) - hot * t_g[k]);
 }
 
 // loss = scale * sum of l[0 .. n), in a fixed order, by NT threads.

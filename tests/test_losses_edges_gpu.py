@@ -1,13 +1,15 @@
 """Calls of the objectives over logits at the edges of what they accept, each
 against its definition in 64 bits."""
 import ctypes as C
+import math
 
 import pytest
 import torch
 
 from dop import losses
 from dop._lib import DOP_BF16, DOP_F32, DopError, check as ok, lib
-from test_losses_gpu import demo, tokens_of
+from test_losses_gpu import (BF16, F32, IDS, TYPES, U, check, demo, gen, last, make_logits, onehot,
+                             tokens_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +91,200 @@ def test_model_operands(cuda):
         m.forward(P, tokens.int())
     assert m.forward(P, tokens, logits=z) is z
     m.close()
+
+
+# ------------------------------------- rows whose maximum is large or far
+# Elements of a row count by their distance from its maximum, which fp32 holds
+# to 2^-24 of itself; one more than 150 ln 2 / below it has probability 0.
+# With |t| <= 150 the power of two's argument c (z - m) is off by 2 u |t| (c
+# rounded, and the product), so a probability's relative error is at most
+#     150 * 2 ln 2 u + 8 u + (V / 128 + 64) u
+# whatever the size of m (the last two as in test_losses_gpu).
+def rel_near(vocab):
+    return (150 * 2 * math.log(2) + 8 + vocab / 128 + 64) * U
+
+
+LOG2E = 1.4426950408889634  # as a temperature: the power of two's factor is 1, |c m| is |m|
+LARGE = [(3e6, LOG2E), (1.6e7, LOG2E), (2e7, LOG2E), (1.3e8, LOG2E), (3e8, LOG2E), (1e9, 1.0),
+         (1e9, 0.1), (3e9, LOG2E), (6e9, 1.0), (1e10, 1.0), (1e12, 0.5), (1e15, 2.0), (1e20, 1.0),
+         (1e30, 3.0), (1e38, 1.0), (1e38, 0.05), (1e5, 2.0 ** -16), (1e15, 2.0 ** 16)]
+
+
+def large_rows(vocab, dtype, base, seed):
+    """Rows around +-base: one value throughout, whole steps of the type below
+    it, ordinary values with one entry there, and rows that are masked by it
+    but for a few entries a little above it."""
+    _, z = make_logits(6, vocab, dtype, 1, 0, seed=seed)
+    b = float(torch.tensor(base).to(dtype))
+    step = b * torch.finfo(dtype).eps
+    k = torch.randint(0, 6, (2, vocab), generator=gen(seed + 1), device="cuda").double()
+    z[0] = -b
+    z[1] = (b - step * k[0]).to(dtype)
+    z[2] = (-b - step * k[1]).to(dtype)
+    z[3, vocab * 2 // 3] = b
+    z[4] = -b
+    z[4, vocab - 2] = -b / 2
+    z[5] = b
+    # a token of the largest value in every row
+    tokens = z.double().argmax(1)
+    return z, tokens
+
+
+def from_maximum(z, tau):
+    """x less its maximum, the maximum, log sum exp of the first, and p."""
+    m = z.double().amax(1)
+    t = (z.double() - m[:, None]) / tau
+    l = torch.logsumexp(t, 1)
+    return t, m / tau, l, torch.exp(t - l[:, None])
+
+
+
+
+@pytest.mark.parametrize("vocab", [300, 9001, 300001])
+@pytest.mark.parametrize("base,tau", LARGE)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+def test_large_rows(cuda, vocab, base, tau, dtype, grad):
+    z, tokens = large_rows(vocab, dtype, base, 401)
+    t, m, l, p = from_maximum(z, tau)
+    rel, n = rel_near(vocab), z.shape[0]
+    hot = onehot(tokens, vocab, torch.ones(n, dtype=torch.bool, device="cuda"))
+    want = t.gather(1, tokens[:, None])[:, 0] - l
+    logp, lse = losses.token_logp(z, tokens, temperature=tau)
+    check("logp", logp, want, rel + last(want, F32))
+    # c, rounded, stands for the temperature where the maximum is not far
+    check("lse", lse, (m + l).float(), rel + 2 * last(m + l, F32))
+
+    old, adv = (want - 0.1).float(), torch.tensor([1.0, -0.5, 0.7, 1.3, 2.0, -1.0], device="cuda")
+    d = -adv.double() * torch.exp(want - old.double())
+    r = losses.policy_loss(z, tokens, old, adv, temperature=tau, scale=0.5, clip_high=0.5, grad_dtype=grad)
+    check("row_loss", r.row_loss, d, d.abs() * (rel + 8 * U) + last(d, F32))
+    ref = 0.5 / tau * d[:, None] * (hot - p)
+    tol = 0.5 / tau * d.abs()[:, None] * (2 * rel + 8 * U) * (p + hot)
+    check("policy dlogits", r.dlogits, ref, tol + last(ref, grad))
+
+
+@pytest.mark.parametrize("vocab", [300, 9001, 300001])
+@pytest.mark.parametrize("base,tau", LARGE)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+@pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
+def test_distill_large_rows(cuda, vocab, base, tau, dtype, grad, tail):
+    """The lists hold some of the entries that have a probability; in row 3
+    an ordinary entry too, and in the last two rows one that the student has
+    at -base and the teacher at probability 0."""
+    z, tokens = large_rows(vocab, dtype, base, 411)
+    z = torch.cat([z, z[3:5]])
+    g = gen(412)
+    z[6:] = torch.randn(2, vocab, generator=g, device="cuda").to(dtype)
+    tokens = torch.cat([tokens, torch.tensor([3, 4], device="cuda")])
+    low = torch.tensor([5, vocab - 1], device="cuda")
+    z[6:].scatter_(1, low[:, None], -base)
+    t, m, l, p = from_maximum(z, tau)
+    n, K = z.shape[0], 6
+    # up to four entries of probability, the row's first largest among them
+    order = torch.topk(t - torch.rand(n, vocab, generator=g, device="cuda") * 1e-3, K, 1).indices
+    order[:, 0] = tokens
+    for i in range(1, K):  # an entry stands once
+        order[:, i] = torch.where((order[:, :i] == order[:, i:i + 1]).any(1), torch.full_like(tokens, -1), order[:, i])
+    order[6:, K - 1] = low
+    top = torch.randn(n, K, generator=g, device="cuda") * tau
+    at = order.clamp(min=0)
+    here = order >= 0
+    # what the student has not got, the teacher has not got either
+    none = ~here | (t.gather(1, at) < -60.0)
+    top = torch.where(none, torch.full_like(top, -math.inf), top)
+    y = top.double() / tau
+    tl = None
+    if tail:
+        tl = torch.logsumexp(y, 1).float() + 0.2
+        # nothing but the listed entries has probability: none is left for the rest
+        alone = torch.zeros(n, vocab, dtype=torch.bool, device="cuda").scatter_(1, at, here)
+        rest = torch.logsumexp((t - l[:, None]).masked_fill(alone, -math.inf), 1)
+        tl = torch.where(rest < -60.0, tl - 0.21, tl)
+    lq = y - (torch.logsumexp(y, 1) if tl is None else tl.double())[:, None]
+    q = torch.where(none, torch.zeros_like(lq), torch.exp(lq))
+    lp = (t - l[:, None]).gather(1, at)
+    zero = torch.zeros_like(lq)
+    row = torch.where(none, zero, q * (torch.where(none, zero, lq) - torch.where(none, zero, lp))).sum(1)
+    size = torch.where(none, zero, q * (1 + lq.abs().nan_to_num(0, 0, 0) + torch.where(none, zero, lp).abs())).sum(1)
+    Q, share = q.sum(1), torch.zeros(n, dtype=torch.float64, device="cuda")
+    if tail:
+        qr = torch.clamp(1 - Q, min=0.0)
+        some = qr > 0
+        qr_ = torch.where(some, qr, torch.ones_like(qr))
+        rest_ = torch.where(some, rest, torch.zeros_like(rest))
+        row = row + torch.where(some, qr * (torch.log(qr_) - rest_), torch.zeros_like(qr))
+        size = size + 1 + torch.where(some, rest_.abs(), torch.zeros_like(qr))
+        share = torch.where(some, qr / torch.exp(rest_), share)
+        Q = Q + qr
+    member = torch.zeros(n, vocab, dtype=torch.bool, device="cuda").scatter_(1, at, here)
+    ref = Q[:, None] * p - share[:, None] * torch.where(member, torch.zeros_like(p), p)
+    qv = torch.zeros_like(p).scatter_add_(1, at, torch.where(here, q, zero))
+    ref = tau * (ref - qv)
+    rel = rel_near(vocab)
+    r = losses.distill_loss(z, order.int().contiguous(), top, teacher_lse=tl, temperature=tau, scale=1.0,
+                            grad_dtype=grad)
+    check("row_loss", r.row_loss, tau * tau * row, tau * tau * size * (rel + 8 * U) + last(tau * tau * row, F32))
+    tol = tau * (p * (2 * rel + 8 * U) * (Q[:, None] + share[:, None] * ~member) + 8 * U * qv)
+    check("dlogits", r.dlogits, ref, tol + last(ref, grad))
+
+
+@pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
+@pytest.mark.parametrize("whole", [0.0, 1.0, 2.0, 6.0])
+def test_distill_between_the_forms(cuda, whole, tail):
+    """Maxima of the listed entries and of the others on both sides of 2^24
+    and a few steps apart."""
+    V, B = 500, 2.0 ** 24
+    _, z = make_logits(4, V, F32, seed=421)
+    k = torch.randint(0, 8, (4, V), generator=gen(422), device="cuda").float()
+    z[:] = (B - 4.0 + whole) - k
+    index = torch.arange(4, dtype=torch.int32, device="cuda").repeat(4, 1).contiguous()
+    z[0, :4] = B + 2.0
+    z[1, :4] = B - 8.0
+    z[2] *= -1.0
+    z[3] = -z[3]
+    z[3, :4] = -B + 6.0
+    tau = LOG2E
+    t, m, l, p = from_maximum(z, tau)
+    top = torch.randn(4, 4, generator=gen(423), device="cuda")
+    y = top.double() / tau
+    tl = torch.logsumexp(y, 1).float() + 0.2 if tail else None
+    lq = y - (torch.logsumexp(y, 1) if tl is None else tl.double())[:, None]
+    q, lp = torch.exp(lq), (t - l[:, None])
+    row, size = (q * (lq - lp[:, :4])).sum(1), (q * (1 + lq.abs() + lp[:, :4].abs())).sum(1)
+    ref = p.clone()
+    share = torch.zeros(4, 1, dtype=torch.float64, device="cuda")
+    if tail:
+        qr, rest = 1 - q.sum(1), torch.logsumexp(lp[:, 4:], 1)
+        row, size = row + qr * (torch.log(qr) - rest), size + 1 + rest.abs()
+        share = (qr / torch.exp(rest))[:, None]
+        ref[:, 4:] -= share * p[:, 4:]
+    ref[:, :4] -= q
+    rel = rel_near(V)
+    r = losses.distill_loss(z, index, top, teacher_lse=tl, temperature=tau, scale=1.0)
+    check("row_loss", r.row_loss, tau * tau * row, tau * tau * size * (rel + 8 * U) + last(tau * tau * row, F32))
+    tol = p * (2 * rel + 8 * U) * (1 + share) + 8 * U
+    check("dlogits", r.dlogits, tau * ref, tau * tol + last(tau * ref, F32))
+
+
+def test_far_rows_among_ordinary_ones_on_several_ctas(cuda):
+    """Masks of -1e9, -1e10 and the lowest value over most of a row, over
+    whole CTAs' shares and over the start, and a row masked altogether."""
+    for dtype in (F32, BF16):
+        for vocab in (1003, 40007, 300001):
+            for low in (-1e9, -1e10, torch.finfo(dtype).min):
+                _, z = make_logits(4, vocab, dtype, 1, 0, seed=431)
+                z[0, : vocab // 2] = low
+                z[1, vocab // 100:] = low
+                z[2, ::2] = low
+                z[3] = low
+                tokens = torch.tensor([vocab - 1, 0, 1, vocab // 3], device="cuda")
+                t, m, l, p = from_maximum(z, 1.0)
+                want = t.gather(1, tokens[:, None])[:, 0] - l
+                rel = rel_near(vocab)
+                logp, lse = losses.token_logp(z, tokens)
+                check("logp", logp, want, rel + last(want, F32))
+                one = torch.ones(4, device="cuda")
+                r = losses.policy_loss(z, tokens, want.float(), one, scale=1.0)
+                hot = onehot(tokens, vocab, one > 0)
+                ref = -torch.exp(want - want.float().double())[:, None] * (hot - p)
+                check("dlogits", r.dlogits, ref, (2 * rel + 8 * U) * (p + hot) + last(ref, dtype))
