@@ -342,6 +342,35 @@ __device__ __forceinline__ void free_columns(uint32_t at) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "n"(N));
 }
 
+// The log-probability adjoint of a row whose lse fp32 does not hold well (above
+// kLseMost, infinite ones too: the rounding of lse to fp32 is an error of p,
+// 2^-24 of lse): from the row's own maximum and sum, by one CTA for the whole
+// row, which may be written in place.  Slow, and out of line: logits in the
+// thousands are rare.
+constexpr float kLseMost = 4096.f;
+template <typename TI, typename TO, int NT>
+__device__ __noinline__ void logp_adjoint_from_row(const TI* z, TO* dz, int V, int token, float c, float hot) {
+  __shared__ float s_m[NT / 32];
+  __shared__ double s_s[NT / 32];
+  const int tid = threadIdx.x;
+  float m = -INFINITY;
+  for (int v = tid; v < V; v += NT) m = fmaxf(m, ld(&z[v]));
+  m = warp_max_redux(m);
+  if ((tid & 31) == 0) s_m[tid >> 5] = m;
+  __syncthreads();
+  for (int w = 0; w < NT / 32; ++w) m = fmaxf(m, s_m[w]);
+  const Form f = form_of(m, c);
+  double s = 0.0;
+  for (int v = tid; v < V; v += NT) s += (double)power(ld(&z[v]), f);
+  s = warp_sum_d(s);
+  if ((tid & 31) == 0) s_s[tid >> 5] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int w = 0; w < NT / 32; ++w) s += s_s[w];
+  const float c_out = (float)(-(double)hot / s);
+  for (int v = tid; v < V; v += NT) st(&dz[v], c_out * power(ld(&z[v]), f) + (v == token ? hot : 0.f));
+}
+
 // A row by a cluster of a.cluster CTAs, of which NT threads own the pieces;
 // distillation has a warp more for the teacher's list.
 template <RowOp OP, Shape S>
@@ -421,6 +450,11 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       if (OP == kLogp && a.logp_lo) a.logp_lo[row] = 0.f;
       if (OP == kPolicy || kList) a.row_loss[row] = 0.f;
     }
+    return;
+  }
+  if (OP == kLogpBwd && fabsf(lse_in) > kLseMost) {
+    if (rank == 0)
+      logp_adjoint_from_row<TI, TO, NT>(z, dz, V, token, a.c, (float)((double)dlogp * a.inv_tau));
     return;
   }
   // every CTA of the cluster has started once this barrier is through: its
@@ -897,17 +931,11 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     }
     return;
   } else if (OP == kLogpBwd) {
-    // 2^(c z - log2(e) lse): the whole part stays in the exponent.  An lse
-    // beyond 1e25 says nothing of p: 0
+    // 2^(c z - log2(e) lse): the whole part stays in the exponent
     const double l2 = (double)lse_in * kLog2e;
     hot = (float)((double)dlogp * a.inv_tau);
-    if (fabsf(lse_in) > 1e25f) {
-      f = {0.f, 1e4f, 0.f};
-      c_out = -hot;
-    } else {
-      f = {a.c, (float)rint(l2), 0.f};
-      c_out = -hot * tc::fast_exp2((float)((double)f.b - l2));
-    }
+    f = {a.c, (float)rint(l2), 0.f};
+    c_out = -hot * tc::fast_exp2((float)((double)f.b - l2));
   } else if (OP == kPolicy) {
     // differences of log-probabilities in double, powers of them in fp32
     const double logp = above(za, rest.m, a.c, a.inv_tau) - ln(rest.s);

@@ -339,9 +339,10 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  *
  * Token log-probabilities: logp[r] = x[tokens[r]] - lse[r]; both are 0 for a
  * skipped row.  Backward: dlogits = dlogp / temperature ([v = token] - p), from
- * the lse of the forward, whose rounding to fp32 p carries (2^-24 |lse|; beyond
- * 1e25 p is taken as 0); rows with dlogp 0 or a token outside [0, vocab) are
- * skipped. */
+ * the lse of the forward, whose rounding to fp32 p carries (2^-24 |lse|); where
+ * |lse| is above 4096, p comes from the row's logits instead (slower: such a
+ * row is read three times by one CTA).  Rows with dlogp 0 or a token outside
+ * [0, vocab) are skipped. */
 int dop_token_logp(int64_t rows, int64_t vocab, int precision, const void* logits, int64_t ld,
                    const int64_t* tokens, const float* weight, double temperature,
                    float* logp, float* lse, void* stream);
@@ -371,7 +372,8 @@ int dop_policy_loss_grad(int64_t rows, int64_t vocab, int precision, const void*
  *   pair_loss = -(1 - label_smoothing) log sigma(margin)
  *               - label_smoothing log sigma(-margin).
  * logp, lse and dlogp [rows] receive the log-probabilities, their log-sum-exp
- * and the loss's adjoint with respect to logp. */
+ * and the loss's adjoint with respect to logp; dlogits comes from the last two
+ * as dop_token_logp_backward has it. */
 int dop_preference_loss_grad(int64_t rows, int64_t vocab, int precision, const void* logits,
                              int64_t ld, const int64_t* tokens, int64_t pairs,
                              const int64_t* seq_off, const float* ref_logp, const float* weight,

@@ -288,3 +288,74 @@ def test_far_rows_among_ordinary_ones_on_several_ctas(cuda):
                 hot = onehot(tokens, vocab, one > 0)
                 ref = -torch.exp(want - want.float().double())[:, None] * (hot - p)
                 check("dlogits", r.dlogits, ref, (2 * rel + 8 * U) * (p + hot) + last(ref, dtype))
+
+
+# ------------------------------ adjoints where fp32 does not hold the row's lse
+@pytest.mark.parametrize("vocab", [300, 9001, 300001])
+@pytest.mark.parametrize("base,tau", [(5e3, 1.0), (1e5, 1.0), (50.0, 1e-3)] + LARGE)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+def test_logp_backward_large_rows(cuda, vocab, base, tau, dtype, grad):
+    """p is the row's softmax whatever its lse: where that is above 4096 it
+    does not come from the fp32 lse, of which 2^-24 would be an error of its
+    own in p.  A far row with entries of -inf is among them."""
+    z, tokens = large_rows(vocab, dtype, base, 441)
+    z[2, 1::3] = -math.inf
+    z[4, 3] = -math.inf
+    tokens = z.double().argmax(1)
+    t, m, l, p = from_maximum(z, tau)
+    rel, n = rel_near(vocab), z.shape[0]
+    logp, lse = losses.token_logp(z, tokens, temperature=tau)
+    g = torch.tensor([1.0, -0.5, 0.7, 1.3, -2.0, 0.25], device="cuda")
+    hot = onehot(tokens, vocab, g != 0)
+    ref = (g.double() / tau)[:, None] * (hot - p)
+    held = (m + l).abs() <= 4096
+    tol = (g.double().abs() / tau)[:, None] * (
+        (rel + U * torch.where(held, (m + l).abs(), torch.zeros_like(m)))[:, None] * p + 4 * U * (p + hot))
+    # c stands for the temperature in p = 2^(c z - lse / ln 2) too: the lse is c's
+    dz = losses.token_logp_backward(z, tokens, lse, g, temperature=tau, grad_dtype=grad)
+    check("dlogits", dz, ref, tol + last(ref, grad))
+    if grad is dtype:  # in the logits' own memory
+        own = torch.empty(z.shape[0] * z.stride(0), dtype=dtype, device="cuda")
+        own = own.view(z.shape[0], z.stride(0))[:, :vocab].copy_(z)
+        losses.token_logp_backward(own, tokens, lse, g, temperature=tau, dlogits=own)
+        assert torch.equal(own, dz)
+
+
+@pytest.mark.parametrize("vocab", [300, 9001, 300001])
+@pytest.mark.parametrize("base,tau", [(5e3, 1.0), (1e9, 1.0), (1e20, 1.0), (1e38, 0.05)])
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+def test_preference_large_rows(cuda, vocab, base, tau, dtype, grad):
+    z, tokens = large_rows(vocab, dtype, base, 451)
+    t, m, l, p = from_maximum(z, tau)
+    rel = rel_near(vocab)
+    off, beta = [0, 2, 3, 4, 6], 0.3
+    logp = t.gather(1, tokens[:, None])[:, 0] - l
+    ref_logp = (logp + torch.randn(6, generator=gen(452), device="cuda")).float()
+    dif = logp - ref_logp.double()
+    margin = beta * torch.stack([dif[0:2].sum() - dif[2], dif[3] - dif[4:6].sum()])
+    dm = -torch.sigmoid(-margin)
+    d = beta * torch.stack([dm[0], dm[0], -dm[0], dm[1], -dm[1], -dm[1]])
+    r = losses.preference_loss(z, tokens, off, ref_logp=ref_logp, temperature=tau, beta=beta, scale=1.0,
+                               grad_dtype=grad)
+    tol_m = beta * 3 * rel
+    check("margin", r.margin, margin, tol_m + last(margin, F32))
+    check("dlogp", r.dlogp, d, beta * (tol_m / 4 + 4 * U) + last(d, F32))
+    hot = onehot(tokens, vocab, d != 0)
+    ref = (d / tau)[:, None] * (hot - p)
+    held = (m + l).abs() <= 4096
+    tol = (beta * (tol_m / 4 + 4 * U) / tau) * (hot + p) + (d.abs() / tau)[:, None] * (
+        (rel + U * torch.where(held, (m + l).abs(), torch.zeros_like(m)))[:, None] * p + 4 * U * (p + hot))
+    check("dlogits", r.dlogits, ref, tol + last(ref, grad))
+
+
+def test_logp_backward_rows_without_a_finite_logit(cuda):
+    """They give NaN, and skipped ones 0, as in the forward."""
+    z = torch.zeros(4, 50, device="cuda")
+    z[0] = -math.inf
+    z[1, 7] = math.inf
+    z[2, 9] = math.nan
+    tokens = torch.tensor([1, 7, 3, 4], device="cuda")
+    logp, lse = losses.token_logp(z, tokens)
+    assert torch.isnan(logp[:3]).all()
+    dz = losses.token_logp_backward(z, tokens, lse, torch.tensor([1.0, 1.0, 1.0, 0.0], device="cuda"))
+    assert torch.isnan(dz[:3]).all() and (dz[3] == 0).all()
