@@ -13,8 +13,8 @@
 //
 // so one kernel serves them: a row is read once into the SM, where its sum of
 // powers is taken (fp32, relative to a whole exponent, so that rescaling is
-// exact), the row's scalars follow (differences of log-probabilities in
-// double), and the adjoint is written from what the SM kept.  What bounds it
+// exact), the row's scalars follow (in double but for a list's q and its
+// coefficients), and the adjoint is written from what the SM kept.  What bounds it
 // is the row's one read and one write; with both sides bf16 the exponentials,
 // two an element at 16 a cycle and SM, come close to that.  Measured on one
 // B200 (6.46 TB/s of measured copy bandwidth), of the bytes read and written
@@ -943,23 +943,24 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
     f = {a.c, (float)rint(l2), 0.f};
     c_out = -hot * tc::fast_exp2((float)((double)f.b - l2));
   } else if (OP == kPolicy) {
-    // differences of log-probabilities in double, powers of them in fp32
-    const double logp = above(za, rest.m, a.c, a.inv_tau) - ln(rest.s);
-    const float ratio = expf((float)(logp - (double)old_logp));
-    const float lo = (float)(1.0 - a.clip_low), hi = (float)(1.0 + a.clip_high);
-    const bool clipped = (adv > 0.f && ratio > hi) || (adv < 0.f && ratio < lo);
-    float l = clipped ? -(adv > 0.f ? hi : lo) * adv : -ratio * adv;
-    float d = clipped ? 0.f : -adv * ratio;
+    // in double: a KL term is a small difference, and a ratio may be beyond
+    // fp32 where the advantage is 0 or the clip holds
+    const double logp = above(za, rest.m, a.c, a.inv_tau) - log((double)rest.s);
+    const double A = (double)adv, ratio = exp(logp - (double)old_logp);
+    const double lo = 1.0 - a.clip_low, hi = 1.0 + a.clip_high;
+    const bool clipped = (A > 0.0 && ratio > hi) || (A < 0.0 && ratio < lo);
+    double l = clipped ? -(A > 0.0 ? hi : lo) * A : -ratio * A;
+    double d = clipped ? 0.0 : -A * ratio;
     if (a.ref_logp) {
-      const float gap = (float)((double)ref_logp - logp), e = expm1f(gap);
-      l += (float)a.kl_coef * (e - gap);
-      d -= (float)a.kl_coef * e;
+      const double gap = (double)ref_logp - logp, e = expm1(gap);
+      l += a.kl_coef * (e - gap);
+      d -= a.kl_coef * e;
     }
     if (tid == 0 && rank == 0) {
-      a.row_loss[row] = w * l;
+      a.row_loss[row] = (float)((double)w * l);
       a.logp[row] = (float)logp;
     }
-    hot = (float)(a.scale * a.inv_tau) * (w * d);
+    hot = (float)(a.scale * a.inv_tau * (double)w * d);
     c_out = -hot / rest.s;
   } else {
     f_in = form_of(all.m, a.c);

@@ -325,8 +325,10 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  *     between the rows; dlogits NULL computes the loss alone (not in
  *     dop_token_logp_backward).  vocab is at most 851,965 (fp32 logits) or
  *     1,703,929 (bf16): DOP_E_UNSUPPORTED above.
- *   - Sums and statistics are fp32 or wider, a row's scalars and the sums over
- *     rows fp64, all in a fixed order: equal inputs in equally aligned rows
+ *   - A row's sum of powers is fp32, its scalars (log-probabilities, ratios,
+ *     margins, what follows of them) and the sums over rows fp64; in
+ *     distillation q, its coefficients and the logarithms of the sums have
+ *     fp32's digits.  All in a fixed order: equal inputs in equally aligned rows
  *     (address modulo 16) give equal bytes.  No call allocates, synchronises
  *     or keeps anything: all of them can be captured in a graph, and calls on
  *     different streams share nothing.

@@ -359,3 +359,80 @@ def test_logp_backward_rows_without_a_finite_logit(cuda):
     assert torch.isnan(logp[:3]).all()
     dz = losses.token_logp_backward(z, tokens, lse, torch.tensor([1.0, 1.0, 1.0, 0.0], device="cuda"))
     assert torch.isnan(dz[:3]).all() and (dz[3] == 0).all()
+
+
+# ------------------------------------------------- a policy row's scalars
+@pytest.mark.parametrize("gap", [1e-4, 1e-3, 1e-2, 0.0])
+@pytest.mark.parametrize("vocab", [97, 40007])
+def test_policy_kl_of_small_gaps(cuda, gap, vocab):
+    """KL alone (advantage 0): exp(gap) - gap - 1 is about gap^2 / 2, and
+    moves by |expm1(gap)| times the log-probability's error e, and by e^2."""
+    n, kl = 6, 0.25
+    _, z = make_logits(n, vocab, F32, seed=501)
+    tokens = tokens_of(n, vocab, 502)
+    t, m, l, p = from_maximum(z, 1.0)
+    lp = t.gather(1, tokens[:, None])[:, 0] - l
+    # (beside the gap, what the fp32 ref_logp leaves: it is an input)
+    sign = torch.tensor([1.0, -1.0, 1.0, -1.0, 0.5, -0.5], device="cuda")
+    ref = (lp + gap * sign).float()
+    g = ref.double() - lp
+    want, d = kl * (torch.expm1(g) - g), -kl * torch.expm1(g)
+    zero = torch.zeros(n, device="cuda")
+    r = losses.policy_loss(z, tokens, lp.float(), zero, ref_logp=ref, kl_coef=kl, scale=1.0)
+    # the log-probability's error, as in test_losses_gpu
+    e = (float(z.abs().max()) * 2 + 8 + vocab / 128 + 64) * U
+    check("row_loss", r.row_loss, want, kl * (torch.expm1(g).abs() * e + e * e) + last(want, F32))
+    hot = onehot(tokens, vocab, zero == 0)
+    check("dlogits", r.dlogits, d[:, None] * (hot - p),
+          (kl * e + 8 * U * d.abs())[:, None] * (hot + p) + (d.abs() * 2 * e)[:, None] * p + last(d[:, None] * p, F32))
+
+
+def test_policy_large_ratios(cuda):
+    """A ratio beyond fp32 beside an advantage of 0, or under the clip, and a
+    KL term whose exponential fp32 does not hold."""
+    V = 40
+    _, z = make_logits(4, V, F32, seed=511)
+    tokens = tokens_of(4, V, 512)
+    t, m, l, p = from_maximum(z, 1.0)
+    lp = t.gather(1, tokens[:, None])[:, 0] - l
+    old = (lp - torch.tensor([100.0, 200.0, 0.0, 95.0], device="cuda")).float()
+    adv = torch.tensor([0.0, 2.0, 0.0, -1e-4], device="cuda")
+    ref = (lp + torch.tensor([0.0, 0.0, 91.0, 0.0], device="cuda")).float()
+    kl = 1e-3
+    ratio, gap = torch.exp(lp - old.double()), ref.double() - lp
+    inside = torch.tensor([1.0, 0.0, 1.0, 1.0], device="cuda")
+    A = adv.double()
+    want = -torch.where(inside > 0, ratio * A, 1.2 * A) + kl * (torch.expm1(gap) - gap)
+    d = -A * ratio * inside - kl * torch.expm1(gap)
+    r = losses.policy_loss(z, tokens, old, adv, ref_logp=ref, kl_coef=kl, scale=1.0)
+    e = (float(z.abs().max()) * 2 + 8 + 64 + 1) * U
+    small = kl * (torch.expm1(gap).abs() * e + e * e)
+    check("row_loss", r.row_loss, want, (ratio * A).abs() * inside * (e + 4 * U) + small + last(want, F32) + 4 * U * A.abs())
+    hot = onehot(tokens, V, inside >= 0)
+    check("dlogits", r.dlogits, d[:, None] * (hot - p),
+          (d.abs() * (3 * e + 8 * U) + kl * e)[:, None] * (hot + p) + last(d[:, None] * p, F32))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [64, 32768])
+def test_policy_scalars_are_of_64_bits(cuda, dtype, vocab):
+    """Rows of zeros, 2^k of them: every power and their sum are exact, so the
+    log-probability -k ln 2 has 64 bits, and a row's loss is off by its own
+    rounding to fp32 alone (2^-40 of the parts is far below that)."""
+    gap = torch.tensor([1e-5, -1e-4, 1e-3, -1e-2, 0.3, -7.0, 1e-6, 0.0], device="cuda")
+    n, kl = gap.numel(), 0.375
+    z = torch.zeros(n, vocab, dtype=dtype, device="cuda")
+    lp = -math.log(vocab)
+    ref, old = lp + gap, lp - gap
+    g, step = ref.double() - lp, lp - old.double()
+    adv = torch.tensor([0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 1.5, -0.75], device="cuda")
+    r = losses.policy_loss(z, tokens_of(n, vocab, 521), old, adv, ref_logp=ref, kl_coef=kl, scale=1.0)
+    A, ratio = adv.double(), torch.exp(step)
+    want = -ratio * A + kl * (torch.expm1(g) - g)
+    check("row_loss", r.row_loss, want, last(want, F32) + 2.0 ** -40 * (ratio * A).abs())
+    d = -ratio * A - kl * torch.expm1(g)
+    hot = (d * (1 - 1 / vocab)).float().double()
+    got = r.dlogits.gather(1, tokens_of(n, vocab, 521)[:, None])[:, 0]
+    # the coefficient and its product with p are rounded to fp32, and the sum
+    # of the two at the token, each once; then to the type
+    check("dlogits", got, hot, d.abs() * 4 * U + last(hot, dtype))
