@@ -611,7 +611,8 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
       const float y = t_q[k];
       const double lq = (tail ? (double)y * a.inv_tau : above(y, t.m, a.c, a.inv_tau)) - tl;
       const float hi = (float)lq;  // q to fp32's last digits: lq rounded, the rest applied
-      const float q = y == -INFINITY ? 0.f : expf(hi) * (1.f + (float)(lq - (double)hi));
+      // (below the smallest fp32 already at -104; there a masked y's rest may be infinite)
+      const float q = y == -INFINITY || lq < -110.0 ? 0.f : expf(hi) * (1.f + (float)(lq - (double)hi));
       t_q[k] = q;
       if (t_g[k] == 0.f) t_g[k] = q;
       qs += (double)q;

@@ -9,7 +9,7 @@ import torch
 from dop import losses
 from dop._lib import DOP_BF16, DOP_F32, DopError, check as ok, lib
 from test_losses_gpu import (BF16, F32, IDS, TYPES, U, check, demo, gen, last, make_logits, onehot,
-                             tokens_of)
+                             teacher, tokens_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -436,3 +436,25 @@ def test_policy_scalars_are_of_64_bits(cuda, dtype, vocab):
     # the coefficient and its product with p are rounded to fp32, and the sum
     # of the two at the token, each once; then to the type
     check("dlogits", got, hot, d.abs() * 4 * U + last(hot, dtype))
+
+
+# ------------------------------------------------ masked entries of a teacher
+@pytest.mark.parametrize("tail", [False, True], ids=["top", "tail"])
+@pytest.mark.parametrize("tau", [0.25, 0.5, 1.0, 2.0])
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e30, -1e9, -1e4])
+def test_distill_masked_teacher(cuda, tail, tau, low):
+    """A teacher's logit at the type's lowest value, or otherwise masked, is
+    one of probability 0: the same loss and adjoint as with -inf, and those
+    bytes."""
+    _, z = make_logits(5, 777, F32, seed=601)
+    index, top, tlse = teacher(z, 12, tau, 602, tail)
+    top[:, 4:9] = low
+    top[4, :11] = low
+    if tail:
+        tlse = torch.logsumexp(top / tau, 1) + 0.1
+    inf = torch.where(top == low, torch.full_like(top, -math.inf), top)
+    a = losses.distill_loss(z, index, top, teacher_lse=tlse, temperature=tau)
+    b = losses.distill_loss(z, index, inf, teacher_lse=tlse, temperature=tau)
+    assert torch.isfinite(b.row_loss).all() and torch.isfinite(b.dlogits).all()
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
