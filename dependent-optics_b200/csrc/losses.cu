@@ -1322,7 +1322,7 @@ void check_rows(int64_t rows, int64_t vocab, int prec, const void* z, int64_t ld
   DOP_REQUIRE(tau >= 0x1p-16 && tau <= 0x1p16, "temperature must lie in [2^-16, 2^16]");
 }
 // dlogits: bf16 or the logits' type; either exactly the logits' memory (same
-// type and stride) or apart from it.
+// type and stride), apart from it, or between its rows.
 void check_grad(int64_t rows, int64_t vocab, int prec, const void* z, int64_t ld, int grad_prec,
                 const void* dz, int64_t ldd) {
   if (!dz) return;
@@ -1330,12 +1330,20 @@ void check_grad(int64_t rows, int64_t vocab, int prec, const void* z, int64_t ld
   DOP_REQUIRE(prec == DOP_F32 || grad_prec == DOP_BF16, "bf16 logits have bf16 dlogits");
   DOP_REQUIRE(ldd >= vocab, "the row stride of dlogits is smaller than vocab");
   DOP_REQUIRE((uintptr_t)dz % elem_bytes(grad_prec) == 0, "misaligned dlogits");
-  if (rows == 0 || (dz == z && prec == grad_prec && ld == ldd)) return;
-  const char *z0 = (const char*)z, *d0 = (const char*)dz;
-  const char* z1 = z0 + ((rows - 1) * ld + vocab) * elem_bytes(prec);
-  const char* d1 = d0 + ((rows - 1) * ldd + vocab) * elem_bytes(grad_prec);
-  DOP_REQUIRE(z1 <= d0 || d1 <= z0,
-              "dlogits overlaps the logits without being the same rows in the same type");
+  if (rows == 0 || (dz == z && prec == grad_prec && (ld == ldd || rows == 1))) return;
+  const int64_t size = elem_bytes(prec), gsize = elem_bytes(grad_prec);
+  const uintptr_t z0 = (uintptr_t)z, d0 = (uintptr_t)dz;
+  const uintptr_t z1 = z0 + ((rows - 1) * ld + vocab) * size, d1 = d0 + ((rows - 1) * ldd + vocab) * gsize;
+  if (z1 <= d0 || d1 <= z0) return;
+  // rows equally far apart may lie between each other: by where a row of
+  // dlogits starts behind the start of a row of logits
+  if (ld * size == ldd * gsize) {
+    const int64_t stride = ld * size;
+    const int64_t behind = d0 >= z0 ? (int64_t)((d0 - z0) % stride)
+                                    : (stride - (int64_t)((z0 - d0) % stride)) % stride;
+    if (behind >= vocab * size && behind + vocab * gsize <= stride) return;
+  }
+  DOP_REQUIRE(false, "dlogits overlaps the logits without being the same rows in the same type");
 }
 
 RowArgs row_args(int64_t vocab, const void* z, int64_t ld, const int64_t* tokens,

@@ -320,7 +320,9 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  *     a row and the matrices need the alignment of an element alone.
  *     `precision` is the logits' type; dlogits has `grad_precision`: DOP_BF16,
  *     or DOP_F32 for fp32 logits.  dlogits may be the logits' own memory when
- *     type and stride are the same (ldd == ld); any other overlap is refused.
+ *     type and stride are the same (ldd == ld; one row has none), and may lie
+ *     between their rows when both are equally many bytes apart; any other
+ *     overlap of the two ranges is refused.
  *     dlogits is ASSIGNED, all of its rows x vocab elements and nothing
  *     between the rows; dlogits NULL computes the loss alone (not in
  *     dop_token_logp_backward).  vocab is at most 851,965 (fp32 logits) or

@@ -458,3 +458,44 @@ def test_distill_masked_teacher(cuda, tail, tau, low):
     assert torch.isfinite(b.row_loss).all() and torch.isfinite(b.dlogits).all()
     for x, y in zip(a, b):
         assert torch.equal(x, y)
+
+
+# ------------------------------------------- dlogits between the logits' rows
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+@pytest.mark.parametrize("vocab,gap", [(7, 0), (1001, 3), (40007, 1)])
+def test_dlogits_between_the_rows(cuda, dtype, grad, vocab, gap):
+    """Logits and dlogits side by side in rows of one buffer, either first:
+    nothing of one is written by the other."""
+    rows = 4
+    size, gsize = torch.finfo(dtype).bits // 8, torch.finfo(grad).bits // 8
+    _, z = make_logits(rows, vocab, dtype, seed=701)
+    tokens, f = tokens_of(rows, vocab, 702), torch.ones(rows, device="cuda")
+    first = (vocab * size + gap * 4 + 3) // 4 * 4
+    for a, b in ((0, first), ((vocab * gsize + gap * 4 + 3) // 4 * 4, 0)):
+        width = (max(a + vocab * size, b + vocab * gsize) + gap + 3) // 4 * 4
+        buf = torch.full((rows * width,), 0x5a, dtype=torch.uint8, device="cuda")
+        zin = torch.as_strided(buf.view(dtype), (rows, vocab), (width // size, 1), a // size).copy_(z)
+        out = torch.as_strided(buf.view(grad), (rows, vocab), (width // gsize, 1), b // gsize)
+        r = losses.policy_loss(zin, tokens, f, f, scale=1.0, dlogits=out)
+        assert torch.equal(zin, z)
+        want = torch.empty(rows * (width // size), dtype=dtype, device="cuda")
+        same = torch.as_strided(want, (rows, vocab), (width // size, 1), 0)  # rows at the same alignment
+        if a % 16 == 0:
+            same.copy_(z)
+            assert torch.equal(losses.policy_loss(same, tokens, f, f, scale=1.0, grad_dtype=grad).dlogits, out)
+        else:
+            x = losses.policy_loss(z, tokens, f, f, scale=1.0, grad_dtype=grad).dlogits
+            check("dlogits", out, x, x.double().abs() * (torch.finfo(grad).eps + 400 * U))
+        rest = torch.as_strided(buf, (rows, width), (width, 1)).clone()
+        rest[:, a:a + vocab * size] = 0x5a
+        rest[:, b:b + vocab * gsize] = 0x5a
+        assert (rest == 0x5a).all()
+
+
+def test_one_row_in_place_under_two_strides(cuda):
+    _, z = make_logits(3, 50, F32, 2, 0, seed=711)
+    row, flat = z[1:2], z[1].unsqueeze(0)
+    tokens, f = tokens_of(1, 50, 712), torch.ones(1, device="cuda")
+    want = losses.policy_loss(row, tokens, f, f).dlogits
+    losses.policy_loss(row, tokens, f, f, dlogits=torch.as_strided(flat, (1, 50), (50, 1)))
+    check("dlogits", row, want, want.double().abs() * 400 * U)
