@@ -8,8 +8,9 @@ import torch
 
 from dop import losses
 from dop._lib import DOP_BF16, DOP_F32, DopError, check as ok, lib
-from test_losses_gpu import (BF16, F32, IDS, TYPES, U, check, demo, gen, last, make_logits, onehot,
-                             teacher, tokens_of)
+from test_losses_gpu import (BF16, F32, IDS, TYPES, U, UNEVEN, check, check_preference, demo, gen, last,
+                             make_logits, onehot, preference_reference, teacher, tokens_of,
+                             uneven_rows)
 
 pytestmark = pytest.mark.gpu
 
@@ -499,3 +500,53 @@ def test_one_row_in_place_under_two_strides(cuda):
     want = losses.policy_loss(row, tokens, f, f).dlogits
     losses.policy_loss(row, tokens, f, f, dlogits=torch.as_strided(flat, (1, 50), (50, 1)))
     check("dlogits", row, want, want.double().abs() * 400 * U)
+
+
+# ------------------------- what the far rows' tests above do not put together
+@pytest.mark.parametrize("vocab", UNEVEN)
+@pytest.mark.parametrize("dtype,grad", TYPES, ids=IDS)
+def test_preference_uneven_rows(cuda, vocab, dtype, grad):
+    z = uneven_rows(vocab, dtype, 801)
+    n = z.shape[0]
+    tokens, off = tokens_of(n, vocab, 802), [0, 4, 9, 13, n]
+    ref = -5.0 + torch.randn(n, generator=gen(803), device="cuda")
+    e = preference_reference(z, tokens, off, ref, None, 1.0, 0.05, 0.1, False, 0.5)
+    r = losses.preference_loss(z, tokens, off, ref_logp=ref, beta=0.05, label_smoothing=0.1, scale=0.5,
+                               grad_dtype=grad)
+    check_preference(r, e, 0.5, grad)
+
+
+@pytest.mark.parametrize("low", [-1e10, -1e9, -3e7])
+@pytest.mark.parametrize("vocab", [500, 40007, 300001])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_distill_with_everything_outside_the_list_masked(cuda, low, vocab, dtype):
+    """The student has its mass on the listed entries, at the start, in the
+    middle and at the end; the others are masked to one far value, so a rest
+    that the teacher holds there costs it their distance."""
+    n, K = 4, 6
+    _, z = make_logits(n, vocab, dtype, 1, 0, seed=811)
+    index = torch.tensor([0, 1, vocab // 2, vocab // 2 + 1, vocab - 2, vocab - 1], device="cuda").repeat(n, 1)
+    keep = z.gather(1, index)
+    z[:] = low
+    z.scatter_(1, index, keep)
+    top = torch.randn(n, K, generator=gen(812), device="cuda")
+    # a rest of 0 in the first two rows, of 0.2 in the others
+    share = torch.tensor([0.0, 0.0, 0.2, 0.2], device="cuda")
+    tl = torch.logsumexp(top, 1) - torch.log1p(-share) - 1e-3 * (share == 0)
+    t, m, l, p = from_maximum(z, 1.0)
+    lp, lq = (t - l[:, None]).gather(1, index), top.double() - tl.double()[:, None]
+    q = torch.exp(lq)
+    qr = torch.clamp(1 - q.sum(1), min=0.0)
+    rest = t[:, 2] - l + math.log(vocab - K)
+    row = (q * (lq - lp)).sum(1) + torch.where(qr > 0, qr * (torch.log(qr) - rest), torch.zeros_like(qr))
+    size = (q * (1 + lq.abs() + lp.abs())).sum(1) + (qr > 0) * (1 + rest.abs())
+    Q = q.sum(1) + qr
+    ref = Q[:, None] * p - (qr / (vocab - K))[:, None]
+    ref.scatter_(1, index, Q[:, None] * p.gather(1, index) - q)
+    rel = rel_near(vocab)
+    r = losses.distill_loss(z, index.int().contiguous(), top, teacher_lse=tl, scale=1.0)
+    check("row_loss", r.row_loss, row, size * (rel + 8 * U) + last(row, F32))
+    # the rest's q is 1 less a sum of q rounded to fp32
+    tol = 2 * rel * Q[:, None] * p + ((qr * (2 * rel) + 8 * U) / (vocab - K))[:, None] + 8 * U * (ref.abs() + p)
+    tol.scatter_add_(1, index, 8 * U * q)
+    check("dlogits", r.dlogits, ref, tol + last(ref, dtype))
