@@ -20,14 +20,14 @@
 // B200 (6.46 TB/s of measured copy bandwidth), of the bytes read and written
 // once:
 //
-//   log-probabilities, 16384 x 32000 bf16, a fifth skipped          145 us  0.90
-//   their adjoint, 4095 x 50001 fp32 to bf16                        209 us  0.91
-//   policy loss, 8192 x 32000 fp32 to bf16, a quarter skipped       235 us  0.86
-//   policy loss, 3001 x 100003 bf16 (rows on odd addresses)         252 us  0.74
-//   preference loss, 16384 x 32000 bf16, three tenths skipped       409 us  0.67
+//   log-probabilities, 16384 x 32000 bf16, a fifth skipped          146 us  0.89
+//   their adjoint, 4095 x 50001 fp32 to bf16                        207 us  0.92
+//   policy loss, 8192 x 32000 fp32 to bf16, a quarter skipped       218 us  0.93
+//   policy loss, 3001 x 100003 bf16 (rows on odd addresses)         255 us  0.73
+//   preference loss, 16384 x 32000 bf16, three tenths skipped       410 us  0.67
 //     (the margins come between two readings of the logits: 0.95 of three passes)
-//   distillation from 64 logits, 32768 x 32000 bf16                 840 us  0.77
-//   with a class for the rest, 128 logits, 2047 x 128000 fp32       420 us  0.77
+//   distillation from 64 logits, 32768 x 32000 bf16                 833 us  0.78
+//   with a class for the rest, 128 logits, 2047 x 128000 fp32       412 us  0.79
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -393,7 +393,7 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
   constexpr bool kKeepPower = sizeof(TI) == 4 && !kOnce;
   constexpr bool kTmem = !kOnce && columns_of(S) > 0;
   constexpr bool kFits = !kOnce && !kTmem;  // every piece has a place of its own
-  constexpr int U = kFits && OP != kDistillRest ? 4 : 2;  // (that one, 16384 x 16001 bf16: 291 us with 4, 276 with 2)
+  constexpr int U = kFits && OP != kDistillRest ? 4 : 2;  // (that one, 16384 x 16001 bf16: 291 us with 4, 274 with 2)
   extern __shared__ __align__(kRingAlign) uint8_t dyn[];
   // of every warp of the cluster
   __shared__ MaxSum s_rest[kMaxCluster * NW];
@@ -404,8 +404,8 @@ __device__ __forceinline__ void vocab_row(const RowArgs& a, const int64_t row, c
   __shared__ double s_q[3];
   __shared__ uint32_t s_tmem;
   // bit k >> kHasShift of an owner: whether its piece k has a listed element
-  // (looked at for every group, the elements' bits where it is set: 426 ->
-  // 413 us for 2047 x 128000 fp32 and 128 entries)
+  // (looked at for every group, the elements' bits where it is set; 16384 x
+  // 16001 bf16: 283 us without it, 274 with; 2047 x 128000 fp32: 400, 409)
   constexpr int kHasShift = S == kAlone ? 2 : 0;
   static_assert(kMovedMost + kRingMost <= 32 << 2 && 2 * kKept <= 32 && kHeldMost <= 32);
   __shared__ uint32_t s_has[tail ? NT : 1];
@@ -1214,12 +1214,13 @@ void allow_shared_memory(const void* kern) {
 // How the rows are laid out over CTAs.  A row whose pieces are kept goes to
 // one narrow or held CTA or to as few wide ones as hold it; more of them where
 // the rows are too few to occupy the SMs (down to 16 KB each).  Both sides, in
-// us: narrow against held for 16384 x 16001 bf16, policy loss 202 / 260,
-// distillation 254 / 344; one held CTA against two narrow ones for 32768 x
-// 32000 bf16, distillation 808 / 883, and against a wide one, 8192 rows, 221 /
-// 237; a wide CTA against four narrow ones for 8192 x 32000 fp32, policy loss
-// 223 / 258; two wide ones against three held ones for 3001 x 100003 bf16,
-// policy loss 250 / 259, and 3000 rows distilled with a rest class 275 / 407.
+// us: narrow against held for 16384 x 16001 bf16, policy loss 209 / 269,
+// distillation 250 / 340, with a rest class 274 / 371; one held CTA against two
+// narrow ones for 32768 x 32000 bf16, distillation 809-827 / 861-867, and
+// against a wide one, 8192 rows, 214 / 228; a wide CTA against four narrow ones
+// for 8192 x 32000 fp32, policy loss 218 / 268; two wide ones against three
+// held ones for 3001 x 100003 bf16, policy loss 253 / 258, and 3000 rows
+// distilled with a rest class 276-281 / 400 (groups of two pieces in both).
 struct Split {
   int cluster, share;  // CTAs per row; pieces per CTA
   Shape shape;

@@ -16,7 +16,9 @@ device.  `weight` [rows] masks and scales rows; a row of weight 0, or whose
 token lies outside [0, vocab), is skipped and its logits are not read.
 
 Work goes to `stream`, or to the device's current stream when it is None; the
-call does not wait for it.  Arguments that do not fit raise DopError.
+call does not wait for it.  A stream given is the caller's to order behind what
+wrote the tensors, which stay in use until it has done the work.  Arguments that
+do not fit raise DopError.
 
     logits = model.forward(params, tokens)
     r = losses.policy_loss(logits, actions, old_logp, advantage, dlogits=logits)
@@ -142,7 +144,8 @@ def token_logp(logits, tokens, *, weight=None, temperature=1.0, stream=None):
 def token_logp_backward(logits, tokens, lse, dlogp, *, temperature=1.0, dlogits=None,
                         grad_dtype=None, stream=None):
     """dlogits from dlogp [rows], the adjoint of `token_logp`'s logp, and the
-    lse it returned.  Rows with dlogp 0 get a row of zeros."""
+    lse it returned.  Rows with dlogp 0 get a row of zeros; those that the
+    forward skipped by their weight need a dlogp of 0."""
     rows, vocab, prec, ld = _matrix(logits, "logits")
     dev = logits.device
     tok = _vector(tokens, "tokens", torch.int64, (rows,), dev)

@@ -356,7 +356,8 @@ class Model:
     def forward(self, params, tokens, logits=None, stream=None):
         """The get: logits fp32 [batch*seq, vocab]; the residual stays in the
         handle for `backward`.  Work goes to `stream`, or to the current stream
-        when it is None.  Every tensor is contiguous and on the device the
+        when it is None; a stream given is the caller's to order behind what
+        wrote the tensors.  Every tensor is contiguous and on the device the
         model was made on: params [n_params] in the model's precision, tokens
         int64 [batch*seq] (in any shape), `logits` (written) as above."""
         import torch

@@ -346,7 +346,8 @@ int dop_gqa_backward_f32_noalloc(int64_t batch, int64_t seq, int64_t heads,
  * the lse of the forward, whose rounding to fp32 p carries (2^-24 |lse|); where
  * |lse| is above 4096, p comes from the row's logits instead (slower: such a
  * row is read three times by one CTA).  Rows with dlogp 0 or a token outside
- * [0, vocab) are skipped. */
+ * [0, vocab) are skipped; a row that the forward skipped by its weight has no
+ * lse, and needs a dlogp of 0. */
 int dop_token_logp(int64_t rows, int64_t vocab, int precision, const void* logits, int64_t ld,
                    const int64_t* tokens, const float* weight, double temperature,
                    float* logp, float* lse, void* stream);
