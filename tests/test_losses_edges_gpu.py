@@ -550,3 +550,37 @@ def test_distill_with_everything_outside_the_list_masked(cuda, low, vocab, dtype
     tol = 2 * rel * Q[:, None] * p + ((qr * (2 * rel) + 8 * U) / (vocab - K))[:, None] + 8 * U * (ref.abs() + p)
     tol.scatter_add_(1, index, 8 * U * q)
     check("dlogits", r.dlogits, ref, tol + last(ref, dtype))
+
+
+@pytest.mark.parametrize("dtype,grad,vocab", [(F32, F32, 851965), (F32, BF16, 851965), (BF16, BF16, 1703929)],
+                         ids=IDS)
+@pytest.mark.parametrize("base", [2e7, 1e10, -1e10])
+def test_far_rows_of_the_largest_vocabulary(cuda, dtype, grad, vocab, base):
+    _, z = make_logits(2, vocab, dtype, 2, 1, seed=821)
+    b = float(torch.tensor(base).to(dtype))
+    z[0] = b
+    z[1, vocab // 3:] = b
+    z[1, : vocab // 3] = b - abs(b) / 4
+    tokens = torch.tensor([5, vocab - 1], device="cuda")
+    t, m, l, p = from_maximum(z, 1.0)
+    want, rel = t.gather(1, tokens[:, None])[:, 0] - l, rel_near(vocab)
+    logp, lse = losses.token_logp(z, tokens)
+    check("logp", logp, want, rel + last(want, F32))
+    one = torch.ones(2, device="cuda")
+    hot = onehot(tokens, vocab, one > 0)
+    ratio = torch.exp(want - want.float().double())
+    r = losses.policy_loss(z, tokens, want.float(), one, scale=1.0, grad_dtype=grad)
+    ref = -ratio[:, None] * (hot - p)
+    check("policy dlogits", r.dlogits, ref, (2 * rel + 8 * U) * (p + hot) + last(ref, grad))
+    d = losses.token_logp_backward(z, tokens, lse, -one, grad_dtype=grad)
+    check("dlogits", d, p - hot, (rel + 8 * U) * (p + hot) + last(p - hot, grad))
+    # all of the teacher's mass on two entries of probability, and a third of it elsewhere
+    index = torch.stack([tokens - 3, tokens], 1).int()
+    for share in (0.0, 1 / 3):
+        tl = torch.full((2,), math.log(2.0) - math.log1p(-share) - 1e-3 * (share == 0), device="cuda")
+        r = losses.distill_loss(z, index, torch.zeros(2, 2, device="cuda"), teacher_lse=tl, scale=1.0, grad_dtype=grad)
+        q = torch.exp(-tl.double())
+        qr = torch.clamp(1 - 2 * q, min=0.0)
+        rest = torch.log(1 - 2 * p.gather(1, tokens[:, None])[:, 0])
+        row = 2 * q * (-tl.double() - want) + torch.where(qr > 0, qr * (torch.log(qr) - rest), torch.zeros_like(qr))
+        check("row_loss", r.row_loss, row, (3 + 2 * want.abs()) * (rel + 8 * U) + last(row, F32))
